@@ -28,7 +28,7 @@ SYMBOLS = [
     "izb_quantize_act", "izb_swiglu_quant", "izb_rmsnorm_quant", "izb_add_norm_quant", "izb_softcap_rows",
     "izb_matmul", "izb_quant_matmul", "izb_gemv", "izb_gemm", "izb_gemm_noalloc", "izb_block_dots", "izb_selfcheck", "izb_matmul_host",
     "izb_moe_route", "izb_moe_route_ex", "izb_moe_sort", "izb_moe_sort_ex", "izb_moe_gateup", "izb_moe_down", "izb_moe_combine",
-    "izb_moe_combine_ex",
+    "izb_moe_combine_ex", "izb_moe_layer", "izb_moe_layer_scratch", "izb_lora_add", "izb_logits_process",
     "izb_tp_range", "izb_tp_add", "izb_tp_unique_id", "izb_tp_create", "izb_tp_create_ex", "izb_tp_wait", "izb_tp_abort", "izb_tp_destroy", "izb_tp_allreduce_rows",
     "izb_tp_reduce_quant_gather", "izb_tp_gather_logits", "izb_p2p_push", "izb_p2p_wait", "izb_p2p_wait_host", "izb_tp_scales_from_ranks",
 ]
@@ -228,6 +228,23 @@ def softcap_rows(c, rows: int, N: int, cap: float, off: int = 0):
     return (_nat or _native()).softcap_rows(c, rows, N, cap, off)
 
 
+def logits_process(logits, out=None, params=None, hist=None, bias=None, mask=None, mask_row=None, want_best: bool = True):
+    """Each request's rules on its row of logits [rows, V] f32 (izb_logits_process), into `out` or in place.  params: [rows, 4] f32 repetition,
+    presence, frequency, temperature; hist: (tokens int32, offsets int32 [rows + 1]); bias: (ids int32, values f32, offsets int32 [rows + 1]);
+    mask: [n_masks, words] int32, a bit per allowed token, with mask_row int32 [rows] (-1: none; not given: mask r for row r).
+    Returns (out, best int32 [rows], logz f32 [rows]), the last two None without want_best."""
+    ht, ho = hist if hist is not None else (None, None)
+    bi, bv, bo = bias if bias is not None else (None, None, None)
+    return (_nat or _native()).logits_process(logits, out, params, ht, ho, bi, bv, bo, mask, mask_row, want_best)
+
+
+def lora_add(A, B, scales, aq, asc, T: int, seg, adapter, out, base=None, c_off: int = 0, ranks=None):
+    """out[t, c_off:c_off+N] += scales[a] * (x[t] A[a]^T) B[a]^T for the T rows, in segments seg [n_seg + 1] int32 with the adapters adapter [n_seg]
+    int32 (izb_lora_add).  A [n, R, K], B [n, N, R] f16 or bf16, contiguous; scales [n] f32; ranks: int32 [n] or None (all R).  base: what is added to,
+    [>= T, N] f32, when it is not `out` itself.  Returns out."""
+    return (_nat or _native()).lora_add(A, B, scales, aq, asc, T, seg, adapter, out, base, c_off, ranks)
+
+
 def matmul(w: Weight, aq, asc, T: int, out=None, c_off: int = 0, acc: int = 0, mat: int = 0):
     """Engine::matmul dispatch: T == 1 GEMV, 2..8 few-row GEMV, else GEMM.  out: [rows, ldc] f32 (default [Mp, N])."""
     return (_nat or _native()).matmul(w.handle.value, w.N, mat, aq, asc, T, out, c_off, acc)
@@ -334,6 +351,13 @@ def moe_down(wd: Weight, hq, hsc, tiles, max_tiles: int, TM: int, swt, S: int):
 
 def moe_combine(x, y, inv, NU: int, sh=None, sgate=None, partial: bool = False):
     return (_nat or _native()).moe_combine(x, y, inv, NU, sh, sgate, partial)
+
+
+def moe_layer(wg: Weight, wu: Weight | None, wd: Weight, aq, asc, logits, NU: int, x=None, out=None, sh=None, e0: int = 0):
+    """The whole expert block of up to 32 tokens in two kernels (izb_moe_layer): logits [T, NE] (or [T, NE + 1] with the shared expert's gate logit
+    last, when sh [T, E] is given) -> out [T, E] = x + the weighted sum over each token's NU experts.  x None: the sum alone; out may be x.
+    wu = None: wg is an interleaved gate | up stack (gateup_weight).  e0: the first expert of the stacks (expert-parallel split)."""
+    return (_nat or _native()).moe_layer(wg.handle.value, wu.handle.value if wu is not None else None, wd.handle.value, wd.N, wd.K, aq, asc, logits, NU, x, out, sh, e0)
 
 
 # ---------------------------------------------------------------------------------------------- tensor parallel

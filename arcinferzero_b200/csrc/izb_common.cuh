@@ -84,6 +84,21 @@ void izb_prof_end(cudaStream_t st);
 
 static inline bool izb_aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
+// Do `rows` x `n` floats at a (row stride lda) and at b (ldb) share bytes without being the same?  Such calls are refused: a thread would read
+// what another has already written.  Windows of different columns of one buffer (equal strides) are apart.
+static inline bool izb_overlap_in_part(const float* a, size_t lda, const float* b, size_t ldb, size_t rows, size_t n) {
+  if (!a || !b) return false;
+  if (rows < 2) lda = ldb = 0;
+  if (a == b && lda == ldb) return false;
+  const uintptr_t a0 = (uintptr_t)a, b0 = (uintptr_t)b, a1 = a0 + ((rows - 1) * lda + n) * 4, b1 = b0 + ((rows - 1) * ldb + n) * 4;
+  if (a0 >= b1 || b0 >= a1) return false;
+  if (rows > 1 && lda == ldb) {
+    const size_t d = (a0 > b0 ? a0 - b0 : b0 - a0) % (lda * 4);
+    if (d >= n * 4 && d + n * 4 <= lda * 4) return false;
+  }
+  return true;
+}
+
 // ---------------------------------------------------------------------------------------------- per-device state
 // The reference drives N GPUs from N threads of ONE process (one Engine per GPU, zero/mgpu/engine_tp.h:825), so everything
 // that belongs to a device's context -- a kernel's opt-in to more than 48 KB of dynamic shared memory, the SM count, the

@@ -22,7 +22,8 @@ namespace {
 
 #define IZB_PY_CALLS(X) \
   X(izb_quantize_act) X(izb_swiglu_quant) X(izb_rmsnorm_quant) X(izb_add_norm_quant) X(izb_softcap_rows) X(izb_matmul) X(izb_quant_matmul) \
-  X(izb_gemv) X(izb_gemm) X(izb_moe_route_ex) X(izb_moe_sort_ex) X(izb_moe_gateup) X(izb_moe_down) X(izb_moe_combine_ex)
+  X(izb_gemv) X(izb_gemm) X(izb_moe_route_ex) X(izb_moe_sort_ex) X(izb_moe_gateup) X(izb_moe_down) X(izb_moe_combine_ex) \
+  X(izb_moe_layer) X(izb_moe_layer_scratch) X(izb_lora_add) X(izb_logits_process)
 
 struct Calls {
 #define X(name) decltype(&name) name##_ = nullptr;
@@ -368,6 +369,143 @@ FN(moe_combine) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- calls that check their tensors: on the current device, of the type, the number of dimensions and the strides that the call reads
+const at::Tensor& checked(PyObject* o, const char* name, std::initializer_list<at::ScalarType> types, int dims) {
+  const at::Tensor& t = tensor(o);
+  bool ok = false;
+  for (at::ScalarType s : types) ok = ok || t.scalar_type() == s;
+  if (!ok) throw torch::TypeError(std::string(name) + ": a tensor of type " + c10::toString(*types.begin()) + " expected, got " + c10::toString(t.scalar_type()));
+  TORCH_CHECK_VALUE(t.dim() == dims, name, ": ", dims, " dimensions expected, got ", t.dim());
+  TORCH_CHECK_VALUE(t.is_cuda(), name, ": a tensor on the GPU expected, got one on ", t.device());
+  TORCH_CHECK_VALUE(t.device().index() == c10::cuda::current_device(), name, ": on ", t.device(), ", but device ", (int)c10::cuda::current_device(), " is current");
+  return t;
+}
+const at::Tensor& whole(PyObject* o, const char* name, std::initializer_list<at::ScalarType> types, int dims) {
+  const at::Tensor& t = checked(o, name, types, dims);
+  TORCH_CHECK_VALUE(t.is_contiguous(), name, ": not contiguous");
+  return t;
+}
+// rows of f32, each contiguous; the row stride
+const at::Tensor& rows_of(PyObject* o, const char* name, int* ld) {
+  const at::Tensor& t = checked(o, name, {at::kFloat}, 2);
+  TORCH_CHECK_VALUE(t.size(1) < 2 || t.stride(1) == 1, name, ": the values of a row are not contiguous");
+  TORCH_CHECK_VALUE(t.size(0) < 2 || (t.stride(0) >= t.size(1) && t.stride(0) <= INT32_MAX), name, ": row stride ", t.stride(0));
+  *ld = t.size(0) < 2 ? (int)t.size(1) : (int)t.stride(0);
+  return t;
+}
+int int32_size(int64_t v, const char* name) {
+  TORCH_CHECK_VALUE(v <= INT32_MAX, name, ": ", v, " is too many");
+  return (int)v;
+}
+// quantised rows: aq [Mp, K] int8, asc [K / 32, Mp] f32
+void quantised_rows(PyObject* aq, PyObject* asc, int64_t K, int64_t T) {
+  const at::Tensor &q = whole(aq, "aq", {at::kChar}, 2), &s = whole(asc, "asc", {at::kFloat}, 2);
+  TORCH_CHECK_VALUE(q.size(1) == K && q.size(0) >= T && s.size(0) == K / 32 && s.size(1) >= T, "aq ", q.sizes(), " and asc ", s.sizes(), " for ", T, " rows of ", K);
+}
+
+// (logits, out, params, hist, hist_off, bias_ids, bias, bias_off, mask, mask_row, want_best): out None = in place
+FN(logits_process) {
+  HANDLE_TH_ERRORS
+  count(n, 11);
+  int ldl = 0, ldo = 0;
+  const at::Tensor& l = rows_of(a[0], "logits", &ldl);
+  PyObject* po = a[1] == Py_None ? a[0] : a[1];
+  const at::Tensor& o = rows_of(po, "out", &ldo);
+  const int64_t rows = l.size(0);
+  const int V = int32_size(l.size(1), "logits");
+  TORCH_CHECK_VALUE(o.size(0) == rows && o.size(1) == V, "out ", o.sizes(), " for logits ", l.sizes());
+  if (a[2] != Py_None) {
+    const at::Tensor& p = whole(a[2], "params", {at::kFloat}, 2);
+    TORCH_CHECK_VALUE(p.size(0) == rows && p.size(1) == 4, "params ", p.sizes(), " for ", rows, " rows ([rows, 4] expected)");
+  }
+  int n_hist = 0, n_bias = 0, words = 0, n_masks = 0;
+  auto offsets = [&](PyObject* o, const char* name) {
+    TORCH_CHECK_VALUE(whole(o, name, {at::kInt}, 1).size(0) == rows + 1, name, ": ", rows + 1, " offsets expected");
+  };
+  if (a[3] != Py_None) {
+    n_hist = int32_size(whole(a[3], "hist", {at::kInt}, 1).size(0), "hist");
+    offsets(a[4], "history offsets");
+  }
+  if (a[5] != Py_None) {
+    n_bias = int32_size(whole(a[5], "bias ids", {at::kInt}, 1).size(0), "bias ids");
+    TORCH_CHECK_VALUE(whole(a[6], "biases", {at::kFloat}, 1).size(0) == n_bias, "as many biases as bias ids expected");
+    offsets(a[7], "bias offsets");
+  }
+  if (a[8] != Py_None) {
+    const at::Tensor& m = whole(a[8], "mask", {at::kInt}, 2);
+    n_masks = int32_size(m.size(0), "mask");
+    words = int32_size(m.size(1), "mask");
+  }
+  if (a[9] != Py_None) TORCH_CHECK_VALUE(whole(a[9], "mask_row", {at::kInt}, 1).size(0) == rows, "mask_row: one per row expected");
+  at::Tensor best, logz;
+  if (PyObject_IsTrue(a[10])) {
+    best = empty({rows}, at::kInt, l.device());
+    logz = empty({rows}, at::kFloat, l.device());
+  }
+  int32_t* pb = best.defined() ? static_cast<int32_t*>(best.data_ptr()) : nullptr;
+  float* pz = logz.defined() ? static_cast<float*>(logz.data_ptr()) : nullptr;
+  call(g.izb_logits_process_, ptr<float>(a[0]), ldl, ptr<float>(po), ldo, int32_size(rows, "logits"), V, ptr<float>(a[2]), ptr<int32_t>(a[3]), ptr<int32_t>(a[4]),
+       n_hist, ptr<int32_t>(a[5]), ptr<float>(a[6]), ptr<int32_t>(a[7]), n_bias, ptr<uint32_t>(a[8]), words, n_masks, ptr<int32_t>(a[9]), pb, pz);
+  return tuple({own(po), pb ? wrap(best) : own(Py_None), pz ? wrap(logz) : own(Py_None)});
+  END_HANDLE_TH_ERRORS
+}
+
+// (A, B, scales, aq, asc, T, seg, adapter, out, base, c_off, ranks): base None = out
+FN(lora_add) {
+  HANDLE_TH_ERRORS
+  count(n, 12);
+  const at::Tensor &A = whole(a[0], "A", {at::kHalf, at::kBFloat16}, 3), &B = whole(a[1], "B", {A.scalar_type()}, 3);
+  const int n_ad = int32_size(A.size(0), "A"), R = int32_size(A.size(1), "A"), K = int32_size(A.size(2), "A"), N = int32_size(B.size(1), "B");
+  TORCH_CHECK_VALUE(B.size(0) == n_ad && B.size(2) == R, "A ", A.sizes(), " and B ", B.sizes(), " ([n, R, K] and [n, N, R] expected)");
+  TORCH_CHECK_VALUE(whole(a[2], "scales", {at::kFloat}, 1).size(0) == n_ad, "scales: one per adapter expected");
+  const int T = num(a[5]), c_off = num(a[10]);
+  quantised_rows(a[3], a[4], K, T);
+  const int n_seg = int32_size(whole(a[7], "adapter", {at::kInt}, 1).size(0), "adapter");
+  TORCH_CHECK_VALUE(whole(a[6], "seg", {at::kInt}, 1).size(0) == (int64_t)n_seg + 1, "seg: ", (int64_t)n_seg + 1, " offsets expected");
+  int ldc = 0, ldb = 0;
+  const at::Tensor& C = rows_of(a[8], "out", &ldc);
+  TORCH_CHECK_VALUE(C.size(0) >= T && c_off >= 0 && C.size(1) >= (int64_t)c_off + N, "out ", C.sizes(), " for ", T, " rows of ", N, " at column ", c_off);
+  const float* base = static_cast<const float*>(C.data_ptr()) + c_off;
+  ldb = ldc;
+  if (a[9] != Py_None) {
+    const at::Tensor& b = rows_of(a[9], "base", &ldb);
+    TORCH_CHECK_VALUE(b.size(0) >= T && b.size(1) >= N, "base ", b.sizes(), " for ", T, " rows of ", N);
+    base = static_cast<const float*>(b.data_ptr());
+  }
+  if (a[11] != Py_None) TORCH_CHECK_VALUE(whole(a[11], "ranks", {at::kInt}, 1).size(0) == n_ad, "ranks: one per adapter expected");
+  call(g.izb_lora_add_, A.scalar_type() == at::kHalf ? IZB_F16 : IZB_BF16, (const void*)A.data_ptr(), (const void*)B.data_ptr(), n_ad, R, ptr<int32_t>(a[11]), ptr<float>(a[2]), N, K,
+       ptr<int8_t>(a[3]), ptr<float>(a[4]), T, extent(a[4], 1), ptr<int32_t>(a[6]), ptr<int32_t>(a[7]), n_seg, base, ldb, static_cast<float*>(C.data_ptr()), ldc, c_off);
+  return own(a[8]);
+  END_HANDLE_TH_ERRORS
+}
+
+// (wg, wu, wd, E, F, aq, asc, logits, NU, x, out, sh, e0): out None = allocate
+FN(moe_layer) {
+  HANDLE_TH_ERRORS
+  count(n, 13);
+  izb_weight *wg = weight(a[0]), *wu = weight(a[1]), *wd = weight(a[2]);
+  const int E = num(a[3]), F = num(a[4]), NU = num(a[8]), e0 = num(a[12]);
+  int ldl = 0;
+  const at::Tensor& l = rows_of(a[7], "logits", &ldl);
+  const int T = int32_size(l.size(0), "logits"), NE = int32_size(l.size(1), "logits") - (a[11] != Py_None ? 1 : 0);
+  quantised_rows(a[5], a[6], E, T);
+  auto block = [&](PyObject* o, const char* name) {
+    const at::Tensor& t = whole(o, name, {at::kFloat}, 2);
+    TORCH_CHECK_VALUE(t.size(0) == T && t.size(1) == E, name, " ", t.sizes(), " ([", T, ", ", E, "] expected)");
+  };
+  if (a[9] != Py_None) block(a[9], "x");
+  if (a[11] != Py_None) block(a[11], "sh");
+  at::Tensor made;
+  if (a[10] == Py_None) made = empty({T, E}, at::kFloat, l.device());
+  else block(a[10], "out");
+  // (the scratch goes back to torch's allocator when this returns, which gives it to later work of this stream only)
+  const at::Tensor scratch = empty({(int64_t)g.izb_moe_layer_scratch_(T, NU, F)}, at::kByte, l.device());
+  call(g.izb_moe_layer_, wg, wu, wd, ptr<int8_t>(a[5]), ptr<float>(a[6]), T, extent(a[6], 1), ptr<float>(a[7]), ldl, NE, NU, e0, ptr<float>(a[11]), ptr<float>(a[9]),
+       made.defined() ? static_cast<float*>(made.data_ptr()) : ptr<float>(a[10]), scratch.data_ptr());
+  return made.defined() ? wrap(made) : own(a[10]);
+  END_HANDLE_TH_ERRORS
+}
+
 // bind(fail, address, {"izb_...": address})
 FN(bind) {
   HANDLE_TH_ERRORS
@@ -405,7 +543,8 @@ PyObject* names(PyObject*, PyObject*) {
 
 #define M(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {M(bind), M(quantize_act), M(swiglu_quant), M(rmsnorm_quant), M(add_norm_quant), M(softcap_rows), M(matmul), M(quant_matmul), M(gemv),
-                         M(gemm), M(moe_route), M(moe_sort), M(moe_gateup), M(moe_down), M(moe_combine), {"names", names, METH_NOARGS, nullptr},
+                         M(gemm), M(moe_route), M(moe_sort), M(moe_gateup), M(moe_down), M(moe_combine), M(moe_layer), M(lora_add),
+                         M(logits_process), {"names", names, METH_NOARGS, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_izb_py", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

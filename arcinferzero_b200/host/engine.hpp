@@ -145,6 +145,27 @@ class Engine {
     cur_K_ = w.K; cur_Mp_ = Mp;
   }
 
+  // adapters of the requests whose rows the quantised activations are, added to the projection's output C (izb_lora_add): the segments' row
+  // offsets seg [n_seg + 1] and adapters [n_seg] on the device
+  struct Adapters {  // d_A [n][R][K], d_B [n][N][R] f16 or bf16, d_ranks (may be null) and d_scales [n], on the device
+    int dtype = IZB_F16, n = 0, R = 0, N = 0, K = 0;
+    const void *A = nullptr, *B = nullptr;
+    const int32_t* ranks = nullptr;
+    const float* scales = nullptr;
+  };
+  void lora_add(const Adapters& l, const int32_t* seg, const int32_t* adapter, int n_seg, float* C, int ldc, int c_off) {
+    if (l.K != cur_K_) throw std::runtime_error("lora_add: the quantised activations do not match these adapters");
+    check(izb_lora_add(l.dtype, l.A, l.B, l.n, l.R, l.ranks, l.scales, l.N, l.K, aq_, asc_, cur_T_, cur_Mp_, seg, adapter, n_seg, C + c_off, ldc, C, ldc, c_off, stream_),
+          "lora_add");
+  }
+  // the expert block of a decode step's rows (izb_moe_layer): x [cur_T][E] += the experts' weighted sum over the quantised activations; scratch
+  // holds moe_scratch(NU, F) bytes
+  size_t moe_scratch(int NU, int F) const { return izb_moe_layer_scratch(cur_T_, NU, F); }
+  void moe_layer(const GpuWeight& gate, const GpuWeight* up, const GpuWeight& down, const float* logits, int ldl, int NE, int NU, const float* sh, float* x, void* scratch) {
+    if (gate.K != cur_K_) throw std::runtime_error("moe_layer: the quantised activations do not match these experts");
+    check(izb_moe_layer(gate.h, up ? up->h : nullptr, down.h, aq_, asc_, cur_T_, cur_Mp_, logits, ldl, NE, NU, 0, sh, x, x, scratch, stream_), "moe_layer");
+  }
+
   // tp_setup (zero/mgpu/engine_tp_shard.h:88): join the communicator; id128 from izb_tp_unique_id on rank 0
   void tp_setup(int nranks, int rank, const void* id128) {
     nranks_ = nranks; rank_ = rank;

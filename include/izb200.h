@@ -61,6 +61,8 @@ extern "C" {
 #define IZB_Q5_K 13
 #define IZB_Q6_K 14
 #define IZB_IQ4_XS 23
+#define IZB_F16 1     /* low-rank adapters (izb_lora_add) */
+#define IZB_BF16 30
 
 /* izb_gemm `impl` */
 /* IZB_GEMM_AUTO, and with it izb_matmul and izb_quant_matmul, may cut a long K (2048 and more) of a plain store into parts when there are few
@@ -198,6 +200,23 @@ int izb_add_norm_quant(float* d_x, const float* d_t, const float* d_w, float eps
  * for r < rows, n < N, in place; row stride ld in floats (the reference passes ld = 0 for one row: any ld is accepted when
  * rows == 1).  cap > 0.  Call it after izb_matmul / izb_gemv on the head's output rows. */
 int izb_softcap_rows(float* d_C, int rows, int ld, int off, int N, float cap, void* stream);
+/* The rules of each request on its row of logits, after the head's product and its soft-cap.  It has no counterpart in the reference.
+ * Per row r and token v, with c = how often v stands in the row's history, in this order, every operation rounded once to f32:
+ *   c > 0:            l = l > 0 ? l / repetition : l * repetition;  l = l - (frequency * c + presence)
+ *   v in the biases:  l = l + bias (of a token that is listed twice the last entry counts)
+ *   mask bit 0:       l = -inf, whatever it was
+ *   temperature > 0:  l = l / temperature (0: a greedy row, its logits stay unscaled)
+ * d_logits [rows][ldl] -> d_out [rows][ldo], V columns each, any alignment; d_out may be d_logits (same stride), else they are apart.
+ * d_params [rows][4]: repetition, presence, frequency, temperature (NULL: neither penalties nor temperature).
+ * d_hist [n_hist], d_hist_off [rows + 1]: row r's history is d_hist[d_hist_off[r] .. d_hist_off[r+1]), tokens in any order and as often as they
+ * came; ids outside 0..V-1 (padding) are skipped.  n_hist = 0: no histories.  d_bias_ids, d_bias [n_bias], d_bias_off [rows + 1]: the biases
+ * likewise.  Offsets past the arrays' ends are cut off there.  d_mask: n_masks rows of mask_words words, bit v & 31 of word v >> 5 = token v is
+ * allowed; d_mask_row[r] = the mask of row r, < 0 or >= n_masks: none (d_mask_row NULL: mask r).  d_mask NULL: no masks.
+ * d_best [rows] (may be NULL) receives the lowest index of a row's largest new logit (NaN is never the largest; a row that nothing is left of: 0),
+ * d_logz [rows] (may be NULL) log(sum(exp(l))) over the row (-inf where nothing is left, NaN where a logit is). */
+int izb_logits_process(const float* d_logits, int ldl, float* d_out, int ldo, int rows, int V, const float* d_params, const int32_t* d_hist,
+                       const int32_t* d_hist_off, int n_hist, const int32_t* d_bias_ids, const float* d_bias, const int32_t* d_bias_off, int n_bias,
+                       const uint32_t* d_mask, int mask_words, int n_masks, const int32_t* d_mask_row, int32_t* d_best, float* d_logz, void* stream);
 
 /* ------------------------------------------------------------------------------------------------ matmul
  * Replaces Engine::matmul / matmul1 (zero/engine.h:1080,1147-1251): C[t][c_off + n] (op)= sum_k A[t][k] W[n][k] for
@@ -221,6 +240,19 @@ int izb_gemv(const izb_weight* w, int mat, const int8_t* d_aq, const float* d_as
              int c_off, int acc, void* stream);
 int izb_gemm(const izb_weight* w, int mat, const int8_t* d_aq, const float* d_asc, int M_rows, int Mp, float* d_C, int ldc,
              int c_off, int acc, int impl, void* stream);
+/* Low-rank adapters of many requests at once beside a projection that they share (no counterpart in the reference): the T rows of a call
+ * come in n_seg segments of consecutive rows, one request each -- a prompt chunk, or the single row of a decode step -- and segment s has the adapter
+ * d_adapter[s] (outside 0..n_adapters-1: none).  With x[t][k] = asc[k/32][t] * aq[t][k], the activations of the projection itself,
+ *   C[t][c_off + n] = base[t][n] + scales[a] * sum_{j < rank_a} B[a][n][j] * (sum_k A[a][j][k] * x[t][k]),   n < N
+ * d_A [n_adapters][R][K], d_B [n_adapters][N][R] in `dtype` (IZB_F16 or IZB_BF16), R % 16 == 0, 16 <= R <= 256, K % 256 == 0; d_scales [n_adapters].
+ * d_ranks [n_adapters] (NULL: all R): adapters of lower rank; their rows of A and columns of B from the rank on are zeros.  Ranks outside 0..R are cut
+ * to it.  d_seg [n_seg + 1]: row offsets, increasing (equal ones: an empty segment); what lies outside 0..T is cut off.  Rows before d_seg[0]
+ * and behind the last segment are left as they were.  base: d_base [T][ldb] (its first column), d_base = d_C + c_off with ldb = ldc to add in place, or
+ * NULL for zeros; rows of segments without an adapter receive the base.  Sums in f32 in an order that depends on the row's place in its segment's
+ * tiles alone, not on other rows.  A, B, aq, asc 16-byte aligned, base and C any f32 address (16-byte aligned rows are faster). */
+int izb_lora_add(int dtype, const void* d_A, const void* d_B, int n_adapters, int R, const int32_t* d_ranks, const float* d_scales, int N, int K,
+                 const int8_t* d_aq, const float* d_asc, int T, int Mp, const int32_t* d_seg, const int32_t* d_adapter, int n_seg, const float* d_base,
+                 int ldb, float* d_C, int ldc, int c_off, void* stream);
 /* Verification mode (the reference's xmx_check idea, zero/engine_setup.h:424): the per-32-block integer dot products
  * themselves, d_dots int32 [M][N][K/32], from the CUDA-core kernel (impl = IZB_GEMM_CORE) or from the tensor-core
  * kernel's accumulators before any scaling (impl = IZB_GEMM_TC).  Both must equal the CPU values bit for bit. */
@@ -306,6 +338,19 @@ int izb_moe_combine(float* d_x, const float* d_y, const int32_t* d_inv, int T, i
  * the shared expert added on one rank only). */
 int izb_moe_combine_ex(float* d_x, const float* d_y, const int32_t* d_inv, int T, int NU, int E, const float* d_sh,
                        const float* d_sgate, int partial, void* stream);
+/* The whole expert block of a decode step's few tokens (T <= 32, T * NU <= 512) in two launches: izb_moe_route's routing of d_logits [T][ldl]
+ * (NE experts, NU choices, ties to the lower id), gate and up with SwiGLU, down, and the combine:
+ *   out[t] = x[t] + sum_k w_k * (h_k Wd_e^T) + sigmoid(logits[t][NE]) * sh[t],   h_k = up * silu(gate) of d_aq / d_asc's row t
+ * wg, wu: stacks [n_mats][F][K], or wu = NULL with an interleaved stack of izb_weight_create_gateup (any tile size: the same stack serves the
+ * prompts' grouped GEMM); wd: [n_mats][K][F], of its own type; Q8_0, Q4_K, Q4_0.  The stacks hold experts [e0, e0 + n_mats) of the NE (a
+ * rank's share in the expert-parallel split; a whole model: e0 = 0, n_mats = NE); choices of other experts add nothing.  d_x NULL: the sum alone (a
+ * rank's partial output); d_sh [T][K] and its gate (logit NE) NULL: no shared expert.  d_x, d_sh and d_out are contiguous [T][K]; d_out may be d_x
+ * or d_sh.  d_scratch: izb_moe_layer_scratch(T, NU, F) bytes, 16-byte aligned, the call's own until it has finished.
+ * h is not quantised to int8 on the way, as the six calls above do (izb_quantize_act between _gateup and _down): results agree with theirs to that rounding,
+ * and are nearer to the exact ones.  A token whose gate * up product is no finite number is NaN. */
+size_t izb_moe_layer_scratch(int T, int NU, int F);
+int izb_moe_layer(const izb_weight* wg, const izb_weight* wu, const izb_weight* wd, const int8_t* d_aq, const float* d_asc, int T, int Mp,
+                  const float* d_logits, int ldl, int NE, int NU, int e0, const float* d_sh, const float* d_x, float* d_out, void* d_scratch, void* stream);
 
 /* ------------------------------------------------------------------------------------------------ tensor parallel
  * tp_range (zero/mgpu/engine_tp_shard.h:68-72): rank r's [begin, end) of `total` in whole `unit`s. */
