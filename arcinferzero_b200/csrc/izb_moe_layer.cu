@@ -4,8 +4,10 @@
 // The six-call path quantises h to int8 in between; here a block of 32 values of h is 23-bit integers Q times a power of two, in three int8 digits
 // (Q = 65536 d1 + 256 d2 + d3), so that the down projection runs on the same integer matrix instruction and h is off by 2^-22 of its block's largest value.
 //
-// Bound by the bytes of the experts that the tokens reach, each read once.  Both kernels work on 16 weight rows x one superblock per warp, straight
-// from global memory into the instruction's registers (lane g = lane / 4, t = lane % 4 holds bytes 8t .. 8t+7 of each block of rows g and g + 8).
+// Bound by the bytes of the experts that the tokens reach, each read once.  Both kernels work on 16 weight rows x one superblock per warp (lane
+// g = lane / 4, t = lane % 4 holds bytes 8t .. 8t+7 of each block of rows g and g + 8).  A warp has a ring of such pieces of its own in shared memory,
+// filled by 16-byte asynchronous copies, and asks for the next piece as soon as it has one in registers, across the borders of experts and channels:
+// 110 to 150 KB per multiprocessor are on their way all the time.
 // Most experts have one or two tokens, for which an instruction with a token per column is mostly empty and a lane repeats a row's scales for all of
 // its blocks.  So the columns are the eight blocks of the superblock instead: the B operand of block b's instruction has the token's values in
 // column b and zeros beside them, eight instructions add up to the 16 x 8 block sums, and lane t scales blocks 2t and 2t + 1 of its two rows -- each
@@ -19,8 +21,9 @@
 namespace {
 
 constexpr int kMaxTokens = 32, kMaxPairs = 512, kMaxExperts = 512, kMaxChoices = 32;
-constexpr int kUpWarps = 8, kSplitK = 4;  // first kernel: two groups of 16 channels x four parts of K
+constexpr int kUpWarps = 16, kSplitK = 8;  // first kernel: two groups of 16 channels x eight parts of K
 constexpr int kDownWarps = 16;
+constexpr int kGroup = 8;                  // tokens of an expert that are dealt with in one go
 constexpr uint32_t kMagic = 0x4B400000u;  // 1.5 * 2^23: accumulators start there and are f32 numbers as they are (|sum| < 2^22)
 
 struct MoeArgs {
@@ -39,8 +42,9 @@ struct Routed {
   float wt[kMaxPairs];
   short id[kMaxPairs];           // the expert's number in the stacks, -1: not here
   uint32_t tokens[kMaxExperts];  // of an expert
-  short list[kMaxExperts];       // experts with tokens, in increasing order
-  int count[17];
+  short list[kMaxPairs];         // experts with tokens, in increasing order, once per kGroup of them ...
+  uint32_t group[kMaxPairs];     // ... and which those are
+  int count[16];
 };
 // One warp: a token's choices in order, ties to the lower id (see izb_moe.cu); the weights' sum in choice order.
 template <int kPer>
@@ -92,7 +96,7 @@ __device__ __forceinline__ void route_token(const MoeArgs& p, int token, Routed&
     if (here) atomicOr(&s.tokens[e], 1u << token);
   }
 }
-// All tokens; the number of experts that have any.  Every thread of the CTA calls it.
+// All tokens; the length of the list.  Every thread of the CTA calls it.
 __device__ int route_all(const MoeArgs& p, Routed& s) {
   const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5, lane = threadIdx.x & 31;
   for (int i = threadIdx.x; i < kMaxExperts; i += blockDim.x) s.tokens[i] = 0u;
@@ -102,18 +106,30 @@ __device__ int route_all(const MoeArgs& p, Routed& s) {
     else route_token<kMaxExperts / 32>(p, t, s);
   }
   __syncthreads();
-  const int groups = (p.n_mats + 31) / 32;  // of 32 experts
-  for (int i = warp; i < groups; i += warps) {
-    const uint32_t has = __ballot_sync(0xFFFFFFFFu, s.tokens[i * 32 + lane] != 0u);
-    if (lane == 0) s.count[i] = __popc(has);
+  const int blocks = (p.n_mats + 31) / 32;  // of 32 experts
+  for (int i = warp; i < blocks; i += warps) {
+    const int n = __reduce_add_sync(0xFFFFFFFFu, (__popc(s.tokens[i * 32 + lane]) + kGroup - 1) / kGroup);
+    if (lane == 0) s.count[i] = n;
   }
   __syncthreads();
   int n = 0;
-  for (int i = 0; i < groups; ++i) {
-    if ((i % warps) == warp) {
-      const bool has = s.tokens[i * 32 + lane] != 0u;
-      const uint32_t all = __ballot_sync(0xFFFFFFFFu, has);
-      if (has) s.list[n + __popc(all & ((1u << lane) - 1u))] = (short)(i * 32 + lane);
+  for (int i = 0; i < blocks; ++i) {
+    if (i % warps == warp) {
+      uint32_t left = s.tokens[i * 32 + lane];
+      const int mine = (__popc(left) + kGroup - 1) / kGroup;
+      int before = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xFFFFFFFFu, before, o);
+        if (lane >= o) before += v;
+      }
+      for (int j = n + before - mine; left; ++j) {
+        uint32_t rest = left;
+        for (int k = 0; k < kGroup; ++k) rest &= rest - 1;  // (0 stays 0)
+        s.list[j] = (short)(i * 32 + lane);
+        s.group[j] = left & ~rest;
+        left = rest;
+      }
     }
     n += s.count[i];
   }
@@ -127,11 +143,6 @@ __device__ __forceinline__ int pair_of(const MoeArgs& p, const Routed& s, int to
 }
 
 // ---------------------------------------------------------------------------------------------- 16 rows x one superblock
-__device__ __forceinline__ uint2 ldg_stream_v2(const void* p) {
-  uint2 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-  return v;
-}
 template <bool kUnsigned>
 __device__ __forceinline__ void mma(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   if (kUnsigned)
@@ -148,17 +159,17 @@ template <int QT>
 struct Raw;
 template <>
 struct Raw<IZB_Q4_K> {
-  static constexpr int kBytes = 144;
+  static constexpr int kBytes = 144, kPitch = 160;  // (40 words: four rows x eight words are on different banks)
   static constexpr bool kMin = true;
   uint2 q[2][4];
   uint4 h[2];
-  __device__ __forceinline__ void load(const uint8_t* r0, const uint8_t* r1, int t) {
-    h[0] = ldg_stream_v4(r0);
-    h[1] = ldg_stream_v4(r1);
+  __device__ __forceinline__ void load(const unsigned char* tile, int g, int t) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      q[0][c] = ldg_stream_v2(r0 + 16 + 32 * c + 8 * t);
-      q[1][c] = ldg_stream_v2(r1 + 16 + 32 * c + 8 * t);
+    for (int r = 0; r < 2; ++r) {
+      const unsigned char* row = tile + (g + 8 * r) * kPitch;
+      h[r] = *reinterpret_cast<const uint4*>(row);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) q[r][c] = *reinterpret_cast<const uint2*>(row + 16 + 32 * c + 8 * t);
     }
   }
   // high nibbles are multiplied where they are, as 16 q: their scale is a 16th
@@ -177,27 +188,28 @@ struct Raw<IZB_Q4_K> {
     for (int r = 0; r < 2; ++r) {
       const uint32_t a = h[r].y >> sh, b = h[r].z >> sh, c = h[r].w >> sh;  // two blocks side by side
       const uint32_t sc = t < 2 ? a & 0x3F3Fu : (c & 0x0F0Fu) | ((a >> 2) & 0x3030u), mn = t < 2 ? b & 0x3F3Fu : ((c >> 4) & 0x0F0Fu) | ((b >> 2) & 0x3030u);
-      const float d = half_bits_to_float(h[r].x & 0xFFFFu), dm = half_bits_to_float(h[r].x >> 16);
-      o.s[r][0] = d * (float)(sc & 0xFFu);
-      o.s[r][1] = d * 0.0625f * (float)(sc >> 8);
-      o.m[r][0] = dm * (float)(mn & 0xFFu);
-      o.m[r][1] = dm * (float)(mn >> 8);
+      // (a byte under the exponent of 2^23 is the number 2^23 + byte, and d * that - d * 2^23 is rounded once: no conversions)
+      const float d = half_bits_to_float(h[r].x & 0xFFFFu), dm = half_bits_to_float(h[r].x >> 16), d0 = -8388608.0f * d, m0 = -8388608.0f * dm;
+      o.s[r][0] = fmaf(d, __uint_as_float(__byte_perm(sc, 0x4B000000u, 0x7440)), d0);
+      o.s[r][1] = fmaf(d * 0.0625f, __uint_as_float(__byte_perm(sc, 0x4B000000u, 0x7441)), d0 * 0.0625f);
+      o.m[r][0] = fmaf(dm, __uint_as_float(__byte_perm(mn, 0x4B000000u, 0x7440)), m0);
+      o.m[r][1] = fmaf(dm, __uint_as_float(__byte_perm(mn, 0x4B000000u, 0x7441)), m0);
     }
   }
 };
 template <>
 struct Raw<IZB_Q8_0> {
-  static constexpr int kBytes = 272;
+  static constexpr int kBytes = 272, kPitch = 288;
   static constexpr bool kMin = false;
   uint2 q[2][8];
   uint32_t h[2];
-  __device__ __forceinline__ void load(const uint8_t* r0, const uint8_t* r1, int t) {
-    h[0] = __ldg(reinterpret_cast<const uint32_t*>(r0) + t);
-    h[1] = __ldg(reinterpret_cast<const uint32_t*>(r1) + t);
+  __device__ __forceinline__ void load(const unsigned char* tile, int g, int t) {
 #pragma unroll
-    for (int c = 0; c < 8; ++c) {
-      q[0][c] = ldg_stream_v2(r0 + 16 + 32 * c + 8 * t);
-      q[1][c] = ldg_stream_v2(r1 + 16 + 32 * c + 8 * t);
+    for (int r = 0; r < 2; ++r) {
+      const unsigned char* row = tile + (g + 8 * r) * kPitch;
+      h[r] = *reinterpret_cast<const uint32_t*>(row + 4 * t);
+#pragma unroll
+      for (int c = 0; c < 8; ++c) q[r][c] = *reinterpret_cast<const uint2*>(row + 16 + 32 * c + 8 * t);
     }
   }
   __device__ __forceinline__ void dots(int (&d)[4], uint2 x, int g) const {
@@ -215,37 +227,121 @@ struct Raw<IZB_Q8_0> {
 };
 __device__ __forceinline__ float number(int d) { return __int_as_float(d) - __uint_as_float(kMagic); }
 
-// ---------------------------------------------------------------------------------------------- gate, up, SwiGLU
-// A CTA takes 32 channels of one expert at a time (one block of h); a warp 16 of them, gate and up, for every fourth superblock.
+// A warp's copies of pieces into its ring.
 template <int QT>
-__global__ void __launch_bounds__(kUpWarps * 32, 2) moe_layer_up_kernel(MoeArgs p) {
+struct Copier {
+  static constexpr int kRowChunks = Raw<QT>::kBytes / 16, kChunks = 16 * kRowChunks, kPer = (kChunks + 31) / 32, kTile = 16 * Raw<QT>::kPitch;
+  uint32_t from[kPer], to[kPer];
+  __device__ __forceinline__ Copier(size_t row_bytes, int lane) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int c = min(lane + 32 * i, kChunks - 1), row = c / kRowChunks, at = 16 * (c % kRowChunks);
+      from[i] = (uint32_t)(row * row_bytes) + at;
+      to[i] = row * Raw<QT>::kPitch + at;
+    }
+  }
+  __device__ __forceinline__ void tile(uint32_t slot, const uint8_t* src, int lane) const {  // 16 rows from `src` on
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (32 * (i + 1) <= kChunks || lane + 32 * i < kChunks)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slot + to[i]), "l"(src + from[i]) : "memory");
+  }
+};
+__device__ __forceinline__ void copies_begun() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// all but the last kLater groups have arrived, for every lane of the warp
+template <int kLater>
+__device__ __forceinline__ void copies_there() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kLater) : "memory");
+  __syncwarp();
+}
+
+// ---------------------------------------------------------------------------------------------- gate, up, SwiGLU
+// A CTA takes 32 channels of one expert at a time (one block of h); a warp 16 of them, gate and up, for every eighth superblock.
+template <int QT>
+struct Up {
+  static constexpr int kSlots = QT == IZB_Q4_K ? 2 : 1, kSlot = 2 * Copier<QT>::kTile;
+  static constexpr size_t kSums = 2 * kUpWarps * kGroup * 32 * sizeof(float), kSmem = kSums + (size_t)kUpWarps * kSlots * kSlot;
+};
+template <int QT>
+__global__ void __launch_bounds__(kUpWarps * 32, 1) moe_layer_up_kernel(MoeArgs p) {
+  extern __shared__ __align__(16) unsigned char smem[];
   __shared__ Routed s;
-  __shared__ float s_sum[kUpWarps][kMaxTokens][32];  // [..][gate row, up row of the warp]
+  constexpr int kSlots = Up<QT>::kSlots, kSlot = Up<QT>::kSlot;
+  auto s_sum = reinterpret_cast<float(*)[kUpWarps][kGroup][32]>(smem);  // [two units][..][..][gate row, up row of the warp]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, half = warp / kSplitK, part = warp % kSplitK;
+  unsigned char* ring = smem + Up<QT>::kSums + (size_t)warp * kSlots * kSlot;
+  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+  const Copier<QT> copier(p.gate_row, lane);
   pdl_wait();
   pdl_launch_next();
-  const int n_exp = route_all(p, s), per = p.F / 32, sbs = p.E / 256;
-  for (int unit = blockIdx.x; unit < n_exp * per; unit += gridDim.x) {
-    const int e = s.list[unit / per], f0 = unit % per * 32;
-    const uint32_t tokens = s.tokens[e];
-    const size_t first = (size_t)e * p.F * (p.joined ? 2 : 1) + (p.joined ? 2 * f0 : f0) + 16 * half + g;
-    const uint8_t* rg = p.wg + first * p.gate_row;
-    const uint8_t* ru = p.joined ? rg + 32 * p.gate_row : p.wu + first * p.gate_row;
+  const int per = p.F / 32, sbs = p.E / 256, entries = route_all(p, s), live = min(kSplitK, sbs);
+
+  // A unit is an entry of the list and a block of 32 channels; a CTA takes every gridDim.x-th.
+  struct Unit {
+    int entry, f0;
+  };
+  auto next = [&](Unit& u, int by) {
+    u.f0 += 32 * by;
+    while (u.f0 >= p.F) {
+      u.f0 -= p.F;
+      ++u.entry;
+    }
+  };
+  Unit asked = {0, 0};  // what is asked for next
+  next(asked, blockIdx.x);
+  Unit unit = asked;
+  int ask_sb = part, ask_slot = 0;
+  const uint8_t *ask_g = nullptr, *ask_u = nullptr;
+  const size_t expert_rows = (size_t)p.F * (p.joined ? 2 : 1);
+  auto open = [&]() {
+    if (asked.entry >= entries) return;
+    const size_t first = s.list[asked.entry] * expert_rows + (p.joined ? 2 * asked.f0 : asked.f0) + 16 * half;
+    ask_g = p.wg + first * p.gate_row + part * Raw<QT>::kBytes;
+    ask_u = p.joined ? ask_g + 32 * p.gate_row : p.wu + first * p.gate_row + part * Raw<QT>::kBytes;
+  };
+  auto ask = [&]() {
+    if (asked.entry < entries) {
+      copier.tile(ring_at + ask_slot * kSlot, ask_g, lane);
+      copier.tile(ring_at + ask_slot * kSlot + Copier<QT>::kTile, ask_u, lane);
+      ask_g += kSplitK * Raw<QT>::kBytes;
+      ask_u += kSplitK * Raw<QT>::kBytes;
+      ask_sb += kSplitK;
+      if (ask_sb >= sbs) {
+        ask_sb = part;
+        next(asked, gridDim.x);
+        open();
+      }
+    }
+    copies_begun();
+    ask_slot = ask_slot + 1 == kSlots ? 0 : ask_slot + 1;
+  };
+  if (part >= sbs) asked.entry = entries;  // (a short K: nothing for this warp)
+  open();
+#pragma unroll
+  for (int i = 0; i < kSlots; ++i) ask();
+
+  for (int buf = 0, slot = 0; unit.entry < entries; next(unit, gridDim.x), buf ^= 1) {
+    const uint32_t tokens = s.group[unit.entry];
     for (int sb = part; sb < sbs; sb += kSplitK) {
-      Raw<QT> wg, wu;
-      const size_t at = (size_t)sb * Raw<QT>::kBytes;
-      wg.load(rg + at, rg + 8 * p.gate_row + at, t);
-      wu.load(ru + at, ru + 8 * p.gate_row + at, t);
+      const int8_t* aq = p.aq + (sb * 256 + g * 32 + 8 * t);
+      const float* asc = p.asc + (size_t)(sb * 8 + 2 * t) * p.Mp;
+      auto values = [&](int token) { return *reinterpret_cast<const uint2*>(aq + token * p.E); };  // (32 rows of at most 2^24 values)
+      auto scale = [&](int token, int i) { return asc[i * p.Mp + token]; };
       uint32_t left = tokens;
-      auto values = [&](int token) { return *reinterpret_cast<const uint2*>(p.aq + (size_t)token * p.E + sb * 256 + g * 32 + 8 * t); };
-      auto scale = [&](int token, int i) { return p.asc[(size_t)(sb * 8 + 2 * t + i) * p.Mp + token]; };
       int token = __ffs(left) - 1;
       uint2 x = values(token);
       float xs[2] = {scale(token, 0), scale(token, 1)};
+      Raw<QT> wg, wu;
+      copies_there<kSlots - 1>();
+      wg.load(ring + slot * kSlot, g, t);
+      wu.load(ring + slot * kSlot + Copier<QT>::kTile, g, t);
+      slot = slot + 1 == kSlots ? 0 : slot + 1;
+      __syncwarp();  // (all lanes have theirs before the slot is filled again)
+      ask();
       Scales cg, cu;
       wg.scales(cg, t);
       wu.scales(cu, t);
-      for (int slot = 0; left; ++slot) {
+      for (int i = 0; left; ++i) {
         left &= left - 1;
         const uint2 x_now = x;
         const float s0 = xs[0], s1 = xs[1];
@@ -280,20 +376,23 @@ __global__ void __launch_bounds__(kUpWarps * 32, 2) moe_layer_up_kernel(MoeArgs 
         const float a = (odd ? v[1] : v[0]) + __shfl_xor_sync(0xFFFFFFFFu, odd ? v[0] : v[1], 1);
         const float b = (odd ? v[3] : v[2]) + __shfl_xor_sync(0xFFFFFFFFu, odd ? v[2] : v[3], 1);
         const float c = (high ? b : a) + __shfl_xor_sync(0xFFFFFFFFu, high ? a : b, 2);
-        float* to = &s_sum[warp][slot][(t >> 1) * 16 + (t & 1) * 8 + g];
+        float* to = &s_sum[buf][warp][i][(t >> 1) * 16 + (t & 1) * 8 + g];
         *to = sb == part ? c : *to + c;
       }
     }
+    // One barrier per unit: the sums of the unit before last have been read before a warp comes to the barrier of the last one.
     __syncthreads();
     // a warp per token: channel f0 + lane
-    const int n_tok = __popc(tokens), live = min(kSplitK, sbs);
-    for (int slot = warp; slot < n_tok; slot += kUpWarps) {
+    const int n_tok = __popc(tokens), f0 = unit.f0;
+    if (warp < n_tok) {
       uint32_t left = tokens;
-      for (int i = 0; i < slot; ++i) left &= left - 1;
-      const int pair = pair_of(p, s, __ffs(left) - 1, e);
+      for (int i = 0; i < warp; ++i) left &= left - 1;
+      const int pair = pair_of(p, s, __ffs(left) - 1, s.list[unit.entry]);
       float gate = 0.0f, up = 0.0f;
-      for (int k = 0; k < live; ++k) {
-        const float* from = s_sum[(lane >> 4) * kSplitK + k][slot];
+#pragma unroll
+      for (int k = 0; k < kSplitK; ++k) {
+        if (k >= live) break;
+        const float* from = s_sum[buf][(lane >> 4) * kSplitK + k][warp];
         gate += from[lane & 15];
         up += from[16 + (lane & 15)];
       }
@@ -315,7 +414,6 @@ __global__ void __launch_bounds__(kUpWarps * 32, 2) moe_layer_up_kernel(MoeArgs 
         p.hsum[(size_t)pair * per + f0 / 32] = unit_of * (float)sum;
       }
     }
-    __syncthreads();
   }
 }
 
@@ -323,51 +421,88 @@ __global__ void __launch_bounds__(kUpWarps * 32, 2) moe_layer_up_kernel(MoeArgs 
 // A CTA takes 16 outputs of all tokens; its warps the experts, each in `splits` parts of F (by F alone, so that a token's sums do not depend on
 // which others the call has).
 template <int QT>
+struct Down {
+  static constexpr int kSlots = QT == IZB_Q4_K ? 3 : 2, kSlot = Copier<QT>::kTile;
+  static size_t smem(int warps, size_t pairs, int splits) { return pairs * splits * 16 * sizeof(float) + (size_t)warps * kSlots * kSlot; }
+};
+template <int QT>
 __global__ void __launch_bounds__(kDownWarps * 32, 1) moe_layer_down_kernel(MoeArgs p) {
-  extern __shared__ float s_y[];  // [T * NU][splits][16]
+  extern __shared__ __align__(16) unsigned char smem[];
   __shared__ Routed s;
+  constexpr int kSlots = Down<QT>::kSlots, kSlot = Down<QT>::kSlot;
+  float* s_y = reinterpret_cast<float*>(smem);  // [T * NU][splits][16]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, g = lane >> 2, t = lane & 3;
+  unsigned char* ring = smem + (size_t)p.T * p.NU * p.splits * 16 * sizeof(float) + (size_t)warp * kSlots * kSlot;
+  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+  const Copier<QT> copier(p.down_row, lane);
   pdl_launch_next();
-  const int n_exp = route_all(p, s), sbs = p.F / 256, per = p.F / 32, items = n_exp * p.splits;
-  bool waited = false;
-  for (int n0 = blockIdx.x * 16; n0 < p.E; n0 += gridDim.x * 16) {
-    Raw<QT> w, next;
-    int item = warp, sb = 0, end = 0;
-    const uint8_t* row = nullptr;
-    auto open = [&]() {  // the item's first superblock and rows
-      if (item >= items) return;
-      const int k = item % p.splits;
-      sb = sbs * k / p.splits;
-      end = sbs * (k + 1) / p.splits;
-      row = p.wd + ((size_t)s.list[item / p.splits] * p.E + n0 + g) * p.down_row;
-    };
-    auto fetch = [&](Raw<QT>& to) { to.load(row + (size_t)sb * Raw<QT>::kBytes, row + 8 * p.down_row + (size_t)sb * Raw<QT>::kBytes, t); };
-    open();
-    if (item < items) fetch(w);
-    if (!waited) {
-      pdl_wait();
-      waited = true;
+  const int splits_log = p.splits - 1, warps_log = __ffs(warps) - 1, items = route_all(p, s) << splits_log, sbs = p.F / 256, per = p.F / 32;  // (one or two splits)
+
+  // A place in a warp's work: 16 outputs, an item (an expert's tokens and a part of F: parts of unlike lengths go round among the warps), a superblock.
+  struct Place {
+    int n0, item, sb, end, k;
+  };
+  auto open = [&](Place& w) {
+    while (w.item >= items && w.n0 < p.E) {
+      w.n0 += gridDim.x * 16;
+      w.item = warp;
+      if (w.item >= items) w.n0 = p.E;  // (fewer items than warps)
     }
-    while (item < items) {
-      const int e = s.list[item / p.splits], k = item % p.splits, now = sb, start = sbs * k / p.splits;
-      uint32_t left = s.tokens[e];
-      if (++sb == end) {
-        item += warps;
-        open();
-      }
-      if (item < items) fetch(next);
-      int pair = pair_of(p, s, __ffs(left) - 1, e);
-      uint2 x[3];
-      float2 hs, hm;
-      auto values = [&]() {
+    w.k = (w.item + (w.item >> warps_log)) & splits_log;
+    w.sb = w.k ? sbs >> 1 : 0;
+    w.end = w.k || !splits_log ? sbs : sbs >> 1;
+  };
+  auto step = [&](Place& w) {
+    if (++w.sb == w.end) {
+      w.item += warps;
+      open(w);
+    }
+  };
+  Place asked = {(int)blockIdx.x * 16, warp, 0, 0, 0};
+  if (warp >= items) asked.n0 = p.E;
+  open(asked);
+  Place now = asked;
+  int ask_slot = 0;
+  auto ask = [&]() {
+    if (asked.n0 < p.E) {
+      copier.tile(ring_at + ask_slot * kSlot, p.wd + ((size_t)s.list[asked.item >> splits_log] * p.E + asked.n0) * p.down_row + (size_t)asked.sb * Raw<QT>::kBytes, lane);
+      step(asked);
+    }
+    copies_begun();
+    ask_slot = ask_slot + 1 == kSlots ? 0 : ask_slot + 1;
+  };
 #pragma unroll
-        for (int d = 0; d < 3; ++d) x[d] = *reinterpret_cast<const uint2*>(p.hq + ((size_t)pair * 3 + d) * p.F + now * 256 + g * 32 + 8 * t);
-        hs = *reinterpret_cast<const float2*>(p.hs + (size_t)pair * per + now * 8 + 2 * t);
-        if (Raw<QT>::kMin) hm = *reinterpret_cast<const float2*>(p.hsum + (size_t)pair * per + now * 8 + 2 * t);
-      };
-      values();
+  for (int i = 0; i < kSlots; ++i) ask();
+  pdl_wait();
+
+  uint2 x[3];
+  float2 hs, hm;
+  int pair = 0;
+  auto values = [&](const Place& w, int token) {
+    pair = pair_of(p, s, token, s.list[w.item >> splits_log]);
+    const int8_t* hq = p.hq + (pair * 3 * p.F + w.sb * 256) + (g * 32 + 8 * t);  // (512 pairs of at most 2^20 values)
+    x[0] = *reinterpret_cast<const uint2*>(hq);
+    x[1] = *reinterpret_cast<const uint2*>(hq + p.F);
+    x[2] = *reinterpret_cast<const uint2*>(hq + 2 * p.F);
+    const int at = pair * per + w.sb * 8 + 2 * t;
+    hs = *reinterpret_cast<const float2*>(p.hs + at);
+    if (Raw<QT>::kMin) hm = *reinterpret_cast<const float2*>(p.hsum + at);
+  };
+  if (now.n0 < p.E) values(now, __ffs(s.group[now.item >> splits_log]) - 1);
+  for (int n0 = blockIdx.x * 16, slot = 0; n0 < p.E; n0 += gridDim.x * 16) {
+    while (now.n0 == n0) {
+      const Place here = now;
+      step(now);
+      Raw<QT> w;
+      copies_there<kSlots - 1>();
+      w.load(ring + slot * kSlot, g, t);
+      slot = slot + 1 == kSlots ? 0 : slot + 1;
+      __syncwarp();
+      ask();
       Scales c;
       w.scales(c, t);
+      uint32_t left = s.group[here.item >> splits_log];
+      const bool first = here.sb == (here.k ? sbs >> 1 : 0);
       while (left) {
         left &= left - 1;
         int d1[4], d2[4], d3[4];
@@ -376,10 +511,8 @@ __global__ void __launch_bounds__(kDownWarps * 32, 1) moe_layer_down_kernel(MoeA
         w.dots(d3, x[2], g);
         const float2 hs_now = hs, hm_now = hm;
         const int pair_now = pair;
-        if (left) {
-          pair = pair_of(p, s, __ffs(left) - 1, e);
-          values();
-        }
+        if (left) values(here, __ffs(left) - 1);
+        else if (now.n0 < p.E) values(now, __ffs(s.group[now.item >> splits_log]) - 1);
         float v[2];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
@@ -392,30 +525,27 @@ __global__ void __launch_bounds__(kDownWarps * 32, 1) moe_layer_down_kernel(MoeA
         float a = (t & 1 ? v[1] : v[0]) + __shfl_xor_sync(0xFFFFFFFFu, t & 1 ? v[0] : v[1], 1);
         a += __shfl_xor_sync(0xFFFFFFFFu, a, 2);
         if (t < 2) {
-          float* to = s_y + ((size_t)pair_now * p.splits + k) * 16 + t * 8 + g;
-          *to = now == start ? a : *to + a;
+          float* to = s_y + ((pair_now << splits_log) + here.k) * 16 + t * 8 + g;
+          *to = first ? a : *to + a;
         }
       }
-      w = next;
     }
     __syncthreads();
     for (int i = threadIdx.x; i < p.T * 16; i += blockDim.x) {
-      const int token = i >> 4, n = n0 + (i & 15);
+      const int token = i >> 4, at = token * p.E + n0 + (i & 15), pr0 = token * p.NU;
+      const float base = p.x ? p.x[at] : 0.0f;
       float v = 0.0f;
+#pragma unroll 4
       for (int k = 0; k < p.NU; ++k) {
-        const int pair = token * p.NU + k;
-        if (s.id[pair] < 0) continue;
-        float y = s_y[(size_t)pair * p.splits * 16 + (i & 15)];
-        for (int j = 1; j < p.splits; ++j) y += s_y[((size_t)pair * p.splits + j) * 16 + (i & 15)];
-        v = fmaf(s.wt[pair], y, v);
+        const float* y = s_y + ((pr0 + k) << splits_log) * 16 + (i & 15);
+        const float sum = splits_log ? y[0] + y[16] : y[0], next = fmaf(s.wt[pr0 + k], sum, v);
+        if (s.id[pr0 + k] >= 0) v = next;
       }
-      const size_t at = (size_t)token * p.E + n;
       if (p.sh) v = fmaf(p.sh[at], 1.0f / (1.0f + expf(-p.logits[(size_t)token * p.ldl + p.NE])), v);
-      p.out[at] = p.x ? p.x[at] + v : v;
+      p.out[at] = p.x ? base + v : v;
     }
     __syncthreads();
   }
-  if (!waited) pdl_wait();
 }
 
 bool takes(const izb_weight* w) { return w->type == IZB_Q4_K || w->type == IZB_Q8_0; }
@@ -440,6 +570,7 @@ extern "C" int izb_moe_layer(const izb_weight* wg, const izb_weight* wu, const i
     IZB_FAIL(IZB_ERR_SHAPE, "moe_layer: a down stack of %d x [%d, %d] for %d experts of %d channels over %d", wd->n_mats, wd->N, wd->K, wg->n_mats, F, E);
   if (T < 1 || NU < 1 || NE < NU || NE > kMaxExperts || NU > kMaxChoices || Mp % 16 || Mp < T || ldl < NE + (d_sh ? 1 : 0))
     IZB_FAIL(IZB_ERR_SHAPE, "moe_layer: T=%d Mp=%d NE=%d NU=%d ldl=%d (NE <= %d, NU <= %d, ldl >= NE, + 1 with a shared expert)", T, Mp, NE, NU, ldl, kMaxExperts, kMaxChoices);
+  if (E > 1 << 20 || F > 1 << 20) IZB_FAIL(IZB_ERR_LIMIT, "moe_layer: %d channels over %d (2^20 at most)", F, E);
   if (T > kMaxTokens || T * NU > kMaxPairs)
     IZB_FAIL(IZB_ERR_LIMIT, "moe_layer: %d tokens x %d experts (up to %d tokens and %d pairs: izb_moe_route, _sort, _gateup, _down and _combine take more)", T, NU, kMaxTokens, kMaxPairs);
   if (!d_scratch) IZB_FAIL(IZB_ERR_ARG, "moe_layer: no scratch");
@@ -460,18 +591,21 @@ extern "C" int izb_moe_layer(const izb_weight* wg, const izb_weight* wu, const i
   p.joined = wg->gu32; p.gate_row = wg->row_bytes; p.down_row = wd->row_bytes;
   p.splits = F >= 512 ? 2 : 1;
   const int sms = izb_sm_count(wg->device), units = (int)(pairs < (size_t)wg->n_mats ? pairs : wg->n_mats) * (F / 32);
-  const int up_grid = units < 2 * sms ? units : 2 * sms;
+  const int up_grid = units < sms ? units : sms;
   // the second kernel: a CTA of 16 warps per multiprocessor, or two of 8 where one round of the former does not do
   const int tiles = E / 16, down_warps = tiles <= sms ? kDownWarps : kDownWarps / 2, most = tiles <= sms ? sms : 2 * sms;
   const int down_grid = tiles < most ? tiles : most;
-  const size_t smem = pairs * p.splits * 16 * sizeof(float);
   cudaStream_t st = (cudaStream_t)stream;
-  auto up = wg->type == IZB_Q4_K ? moe_layer_up_kernel<IZB_Q4_K> : moe_layer_up_kernel<IZB_Q8_0>;
-  auto down = wd->type == IZB_Q4_K ? moe_layer_down_kernel<IZB_Q4_K> : moe_layer_down_kernel<IZB_Q8_0>;
-  constexpr size_t kMaxSmem = (size_t)kMaxPairs * 2 * 16 * sizeof(float);
-  IZB_SMEM_OPTIN(moe_layer_down_kernel<IZB_Q4_K>, kMaxSmem, wd->device);
-  IZB_SMEM_OPTIN(moe_layer_down_kernel<IZB_Q8_0>, kMaxSmem, wd->device);
-  IZB_LAUNCH("moe_layer_up", st, izb_launch_pdl(up, up_grid, kUpWarps * 32, 0, st, p));
-  IZB_LAUNCH("moe_layer_down", st, izb_launch_pdl(down, down_grid, down_warps * 32, smem, st, p));
+  const bool up4 = wg->type == IZB_Q4_K, down4 = wd->type == IZB_Q4_K;
+  const size_t up_smem = up4 ? Up<IZB_Q4_K>::kSmem : Up<IZB_Q8_0>::kSmem;
+  const size_t down_smem = down4 ? Down<IZB_Q4_K>::smem(down_warps, pairs, p.splits) : Down<IZB_Q8_0>::smem(down_warps, pairs, p.splits);
+  IZB_SMEM_OPTIN(moe_layer_up_kernel<IZB_Q4_K>, Up<IZB_Q4_K>::kSmem, wg->device);
+  IZB_SMEM_OPTIN(moe_layer_up_kernel<IZB_Q8_0>, Up<IZB_Q8_0>::kSmem, wg->device);
+  IZB_SMEM_OPTIN(moe_layer_down_kernel<IZB_Q4_K>, Down<IZB_Q4_K>::smem(kDownWarps, kMaxPairs, 2), wg->device);
+  IZB_SMEM_OPTIN(moe_layer_down_kernel<IZB_Q8_0>, Down<IZB_Q8_0>::smem(kDownWarps, kMaxPairs, 2), wg->device);
+  auto up = up4 ? moe_layer_up_kernel<IZB_Q4_K> : moe_layer_up_kernel<IZB_Q8_0>;
+  auto down = down4 ? moe_layer_down_kernel<IZB_Q4_K> : moe_layer_down_kernel<IZB_Q8_0>;
+  IZB_LAUNCH("moe_layer_up", st, izb_launch_pdl(up, up_grid, kUpWarps * 32, up_smem, st, p));
+  IZB_LAUNCH("moe_layer_down", st, izb_launch_pdl(down, down_grid, down_warps * 32, down_smem, st, p));
   return IZB_OK;
 }
