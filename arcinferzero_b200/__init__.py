@@ -28,7 +28,7 @@ SYMBOLS = [
     "izb_quantize_act", "izb_swiglu_quant", "izb_rmsnorm_quant", "izb_add_norm_quant", "izb_softcap_rows",
     "izb_matmul", "izb_quant_matmul", "izb_gemv", "izb_gemm", "izb_gemm_noalloc", "izb_block_dots", "izb_selfcheck", "izb_matmul_host",
     "izb_moe_route", "izb_moe_route_ex", "izb_moe_sort", "izb_moe_sort_ex", "izb_moe_gateup", "izb_moe_down", "izb_moe_combine",
-    "izb_moe_combine_ex", "izb_moe_layer", "izb_moe_layer_scratch", "izb_lora_add", "izb_logits_process",
+    "izb_moe_combine_ex", "izb_moe_layer", "izb_moe_layer_scratch", "izb_lora_add", "izb_lora_scratch", "izb_logits_process",
     "izb_tp_range", "izb_tp_add", "izb_tp_unique_id", "izb_tp_create", "izb_tp_create_ex", "izb_tp_wait", "izb_tp_abort", "izb_tp_destroy", "izb_tp_allreduce_rows",
     "izb_tp_reduce_quant_gather", "izb_tp_gather_logits", "izb_p2p_push", "izb_p2p_wait", "izb_p2p_wait_host", "izb_tp_scales_from_ranks",
 ]

@@ -2,16 +2,18 @@
 // or none,
 //   u[t][j] = sum_k A[j][k] x[t][k],  x[t][k] = asc[k / 32][t] aq[t][k],      C[t][c_off + n] = base[t][n] + scale * sum_j B[n][j] u[t][j].
 //
-// Bound by bytes: the adapters' for decode rows, base in and outputs out for prompts (rank 64 over 17408 outputs: 64 operations per byte).  One kernel does
-// both products, so that u never goes to memory and a call is one launch: a cluster of CTAs per tile of rows of one segment, each with a share of K for the
-// first product; the partial sums meet in distributed shared memory, and each CTA goes on with its share of N.  The work is on mma.sync with 16-bit operands:
-// the int8 values are exact in them, so the first product is exact up to its f32 sums; u enters the second one in pieces that add up to 22 bits or more of
-// it (f16: two, after a power of two per row that brings the row's largest value below 2^14; bf16: three).  (The tcgen05 path would want 128 rows of one adapter
-// per tile and its accumulators back through registers for the base; the tensor pipe is a tenth busy as it is.)
+// Bound by bytes: the adapters' for decode rows, base in and outputs out for prompts (rank 64 over 17408 outputs: 64 operations per byte).  The work is on
+// mma.sync with 16-bit operands: the int8 values are exact in them, so the first product is exact up to its f32 sums; u enters the second one in pieces that
+// add up to 22 bits or more of it (f16: two, after a power of two per row that brings the row's largest value below 2^14; bf16: three).  (The tcgen05 path
+// would want 128 rows of one adapter per tile and its accumulators back through registers for the base; the tensor pipe is a third busy as it is.)
 //
-// Two forms.  lora_few_kernel: tiles of up to 8 rows, ranks (then outputs) on the instruction's 16-wide side and rows on the 8-wide one.
-// lora_rows_kernel: tiles of up to 64 rows; in the second product the rows are on the 16-wide side, and the column order within 16 outputs is chosen so that
-// a lane has four neighbouring ones: 16-byte loads of the base and stores.
+// Two forms.  Decode rows (lora_few_kernel, up to 8 rows per segment on average): one launch and no memory for u.  A cluster of CTAs per tile of up to 8 rows
+// of a segment, each with a share of K; the partial sums meet in distributed shared memory, and each CTA goes on with its share of the outputs.  Ranks, then
+// outputs, are on the instruction's 16-wide side and rows on the 8-wide one.
+// Prompts: tiles of up to 64 rows.  lora_inner_kernel makes u's pieces (a cluster per tile, a share of K each) and a list of the tiles; lora_outer_kernel
+// deals out steps of 64 rows x 64 outputs in equal stretches.  (Both in one kernel, a cluster per tile, left the last of 3.5 rounds half empty and the
+// memory idle during the first product: 312 us for 8192 x 5120 -> 17408 at rank 64.)  In the second product the order of columns within 16 outputs is chosen so
+// that a lane has four neighbouring ones: 16-byte copies of the base and stores.
 #include <cuda_bf16.h>
 
 #include "izb_common.cuh"
@@ -35,9 +37,10 @@ struct Tile {
   float scale;
 };
 template <int kRows>
-__device__ __forceinline__ Tile find_tile(const LoraArgs& p, int tile, Tile* s_tile, int* s_sum) {
+__device__ __forceinline__ Tile find_tile(const LoraArgs& p, int tile, Tile* s_tile, int* s_sum, int* seen = nullptr) {  // `seen`: of a tile too many, how many there are
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid == 0) s_tile->rows = 0;
+  const int asked = tile;
   for (int s0 = 0; s0 < p.n_seg; s0 += kThreads) {
     const int s = s0 + tid;
     int lo = 0, hi = 0, a = -1, rank = 0;
@@ -79,6 +82,7 @@ __device__ __forceinline__ Tile find_tile(const LoraArgs& p, int tile, Tile* s_t
     if (tile < total) break;
     tile -= total;
   }
+  if (seen) *seen = asked - tile;
   return *s_tile;
 }
 
@@ -390,33 +394,36 @@ __global__ void __launch_bounds__(kThreads, 2) lora_few_kernel(LoraArgs p) {
 }
 
 // ---------------------------------------------------------------------------------------------- up to 64 rows
-constexpr int kRows = 64, kRowsCluster = 8, kOwn = kRows / kRowsCluster;  // a CTA joins the sums of kOwn rows
-constexpr int kCols = 64;                                                  // outputs of a step of the second product
-// u's pieces and B's tiles: rows of R rounded up to 32 values, in 16-byte chunks; where a row is a multiple of 128 bytes odd rows have the halves of
-// their 128-byte lines changed over, so that two neighbouring rows' 64 bytes lie on different banks.  The same with A's tiles.
+constexpr int kRows = 64;         // rows of a tile
+constexpr int kCols = 64;         // outputs of a step of the second product
+// u's pieces, A's and B's tiles: rows of whole 64 bytes in 16-byte chunks; where a row is a multiple of 128 bytes odd rows have the halves of their
+// 128-byte lines changed over, so that two neighbouring rows' 64 bytes lie on different banks.
 struct RowsPlan {
-  int groups;                         // warps side by side on ranks in the first product, 32 ranks each; the others share its blocks of K
-  int ld, swap;                       // a row's 16-bit values; what odd rows' chunk numbers are xored with
-  int stages1, stages2;               // of asynchronous copies, in the first product and in the second
+  int groups, parts;                  // warps by ranks (64 each) and by blocks of K in the first product; two more by rows (32 each)
+  int ld, swap;                       // a row of u or B in 16-bit values (a multiple of 32); what odd rows' chunk numbers are xored with
+  int stages2;                        // of asynchronous copies in the second product (three in the first)
   uint32_t stage1, stage2;            // bytes: activations | their scales | A's tile; B's tile | base
-  uint32_t first, all, total;         // where the stages (over them the partial sums) and the CTAs' sums are, behind the pieces
-  RowsPlan(int R, bool bf16) {
-    groups = R <= 32 ? 1 : R <= 64 ? 2 : R <= 128 ? 4 : 8;
-    const int parts = kWarps / groups;
+  uint32_t all, total1;               // first product: the CTAs' sums lie behind the stages and, over them, the warps' sums
+  uint32_t pieces, total2;            // second product: u's pieces, then stages
+  uint32_t at_tiles, at_factors, at_pieces;  // scratch: number of tiles | Tile each | 64 factors each | pieces each
+  RowsPlan(int R, bool bf16, size_t tiles) {
+    groups = R <= 64 ? 1 : R <= 128 ? 2 : 4;
+    parts = kWarps / 2 / groups;
     ld = (R + 31) / 32 * 32;
     swap = ld % 64 ? 0 : 4;
-    first = (bf16 ? 3 : 2) * kRows * ld * 2;
-    stages1 = R <= 32 ? 2 : 3;
-    stages2 = R <= 128 ? 3 : 2;
     stage1 = parts * (kRows * 32 + kRows * 4 + R * 64);
+    const uint32_t part = (uint32_t)parts * R * kRows * 4;
+    all = part > 3 * stage1 ? part : 3 * stage1;
+    total1 = all + (uint32_t)R * kRows * 4;
+    pieces = (bf16 ? 3 : 2) * kRows * ld * 2;
     stage2 = kCols * ld * 2 + kRows * kCols * 4;
-    const uint32_t part = (uint32_t)parts * R * kRows * 4, sums = (uint32_t)kRowsCluster * R * kOwn * 4;
-    const uint32_t early = (stages2 - 1) * stage2;  // (in use before the sums have been read)
-    all = first + (part > early ? part : early);
-    total = all + sums;
-    if (total < first + stages1 * stage1) total = first + stages1 * stage1;
-    if (total < first + stages2 * stage2) total = first + stages2 * stage2;
+    stages2 = R <= 128 ? 3 : 2;
+    total2 = pieces + stages2 * stage2;
+    at_tiles = 16;
+    at_factors = (uint32_t)(at_tiles + tiles * sizeof(Tile) + 15) / 16 * 16;
+    at_pieces = (uint32_t)(at_factors + tiles * kRows * 4);
   }
+  size_t scratch(size_t tiles) const { return at_pieces + tiles * pieces; }
 };
 template <int kN>
 __device__ __forceinline__ void copies_there() { asm volatile("cp.async.wait_group %0;" ::"n"(kN) : "memory"); }
@@ -429,98 +436,99 @@ __device__ __forceinline__ void copy16(uint32_t to, const void* from) { asm vola
 __device__ __forceinline__ void copy4(uint32_t to, const void* from) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory"); }
 __device__ __forceinline__ void copies_begun() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 
-// kRegs: the ranks are 64 at most, and a warp holds its rows' pieces in registers through the second product
-template <bool kBf16, bool kVec, bool kRegs>
-__global__ void __launch_bounds__(kThreads, 2) lora_rows_kernel(LoraArgs p, RowsPlan plan) {
+// The first product: u's pieces, rows' factors and the tile's place, into scratch.
+template <bool kBf16>
+__global__ void __launch_bounds__(kThreads, 2) lora_inner_kernel(LoraArgs p, RowsPlan plan, unsigned char* scratch) {
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ Tile s_tile;
   __shared__ int s_sum[kWarps];
-  __shared__ float s_factor[kRows];
-  uint16_t* s_u = reinterpret_cast<uint16_t*>(smem);              // [piece][64][ld]
-  float* s_part = reinterpret_cast<float*>(smem + plan.first);    // [K part][R][64 rows]
-  float* s_all = reinterpret_cast<float*>(smem + plan.all);       // [CTA][R][kOwn]
-  const int ld = plan.ld;
-  const int rank_of_cta = blockIdx.x % kRowsCluster, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  float* s_part = reinterpret_cast<float*>(smem);              // [K part][R][64 rows]
+  float* s_all = reinterpret_cast<float*>(smem + plan.all);    // [CTA][R][rows that the CTA joins]
+  const int index = blockIdx.x / p.cluster, rank_of_cta = blockIdx.x % p.cluster, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   cluster_arrive();
-  pdl_launch_next();
   pdl_wait();
-  const Tile tile = find_tile<kRows>(p, blockIdx.x / kRowsCluster, &s_tile, s_sum);
+  pdl_launch_next();
+  int seen = 0;
+  const Tile tile = find_tile<kRows>(p, index, &s_tile, s_sum, &seen);
+  if (tid == 0 && rank_of_cta == 0) {
+    if (tile.rows) reinterpret_cast<Tile*>(scratch + plan.at_tiles)[index] = tile;
+    if (blockIdx.x + p.cluster == gridDim.x) *reinterpret_cast<int*>(scratch) = tile.rows ? index + 1 : seen;
+  }
   if (!tile.rows || tile.rank == 0) {
-    if (tile.rows) copy_base(p, tile, rank_of_cta);
     cluster_wait();
     return;
   }
   const uint16_t* A = p.A + (size_t)tile.adapter * p.R * p.K;
-  const uint16_t* B = p.B + (size_t)tile.adapter * p.N * p.R;
   const int rank = (tile.rank + 15) & ~15;
-  const uint32_t stages_at = (uint32_t)__cvta_generic_to_shared(smem) + plan.first;
 
-  // ---- u: a warp has 32 ranks x 64 rows, and every parts-th 32-block of the CTA's share of K; `parts` blocks per stage
-  const int parts = kWarps / plan.groups, part = warp / plan.groups, j0 = warp % plan.groups * 32;
+  // ---- a warp has 64 ranks x 32 rows, and every parts-th 32-block of the CTA's share of K; `parts` blocks per stage
+  const int parts = plan.parts, part = warp % parts, r0 = (warp / parts & 1) * 32, j0 = warp / (2 * parts) * 64;
   {
-    const int kb0 = share(p.K / 32, kRowsCluster, rank_of_cta), kb1 = share(p.K / 32, kRowsCluster, rank_of_cta + 1), steps = (kb1 - kb0 + parts - 1) / parts;
+    const int kb0 = share(p.K / 32, p.cluster, rank_of_cta), kb1 = share(p.K / 32, p.cluster, rank_of_cta + 1), steps = (kb1 - kb0 + parts - 1) / parts;
     const int row_log = __ffs(parts) + 1, swap = parts > 1 ? 4 : 0;  // a row of A's tile: 2^row_log chunks
-    const uint32_t scales_at = parts * kRows * 32, a_at = scales_at + parts * kRows * 4;
+    const uint32_t stages_at = (uint32_t)__cvta_generic_to_shared(smem), scales_at = parts * kRows * 32, a_at = scales_at + parts * kRows * 4;
+    // (rows past the tile's: the last one again, which nobody reads)
+    const int8_t* x_from = p.aq + (size_t)(tile.row + min((tid >> 1) & (kRows - 1), tile.rows - 1)) * p.K + (kb0 + (tid >> 7)) * 32 + (tid & 1) * 16;
+    const float* s_from = p.asc + (size_t)(kb0 + (tid >> 6)) * p.Mp + tile.row + min(tid & (kRows - 1), tile.rows - 1);
+    const int a_c = tid & ((1 << row_log) - 1), a_j = tid >> row_log, a_step = kThreads >> row_log;
+    const uint16_t* a_from = A + (size_t)a_j * p.K + kb0 * 32 + a_c * 8;
+    const uint32_t a_to = a_at + ((a_j << row_log) + (a_c ^ (a_j & 1 ? swap : 0))) * 16;  // (a_step is even: the rows of a thread are all odd or all even)
     auto ask = [&](int step, int stage) {
       if (step < steps) {
         const uint32_t to = stages_at + stage * plan.stage1;
-        const int kb = kb0 + step * parts, blocks = min(parts, kb1 - kb);
-        for (int i = tid; i < blocks * kRows * 2; i += kThreads) {  // (rows past the tile's: the last one again, which nobody reads)
-          const int r = min((i >> 1) & (kRows - 1), tile.rows - 1);
-          copy16(to + i * 16, p.aq + (size_t)(tile.row + r) * p.K + (kb + (i >> 7)) * 32 + (i & 1) * 16);
-        }
-        for (int i = tid; i < blocks * kRows; i += kThreads)
-          copy4(to + scales_at + i * 4, p.asc + (size_t)(kb + (i >> 6)) * p.Mp + tile.row + min(i & (kRows - 1), tile.rows - 1));
-        for (int i = tid; i < rank << row_log; i += kThreads) {
-          const int j = i >> row_log, c = i & ((1 << row_log) - 1);
-          if (c < blocks * 4) copy16(to + a_at + ((j << row_log) + (c ^ (j & 1 ? swap : 0))) * 16, A + (size_t)j * p.K + kb * 32 + c * 8);
+        const int blocks = min(parts, kb1 - kb0 - step * parts), k = step * parts * 32;
+        for (int i = tid; i < blocks * kRows * 2; i += kThreads) copy16(to + i * 16, x_from + k + (i - tid) / 4);
+        if (tid < blocks * kRows) copy4(to + scales_at + tid * 4, s_from + (size_t)(step * parts) * p.Mp);
+        if (a_c < blocks * 4) {
+          const uint16_t* from = a_from + k;
+          for (int j = a_j, i = 0; j < rank; j += a_step, ++i, from += (size_t)a_step * p.K) copy16(to + a_to + i * (kThreads * 16), from);
         }
       }
       copies_begun();
     };
-    float acc[2][8][4] = {};
-    const bool one = j0 < rank, two = j0 + 16 < rank;
-    for (int i = 0; i < plan.stages1 - 1; ++i) ask(i, i);
+    float acc[4][4][4] = {};
+    ask(0, 0);
+    ask(1, 1);
     for (int step = 0, stage = 0; step < steps; ++step) {
-      copies_there(plan.stages1 - 2);
+      copies_there<1>();
       __syncthreads();
-      ask(step + plan.stages1 - 1, stage == 0 ? plan.stages1 - 1 : stage - 1);
-      const unsigned char* here = smem + plan.first + stage * plan.stage1;
-      stage = stage + 1 == plan.stages1 ? 0 : stage + 1;
-      if (!one || kb0 + step * parts + part >= kb1) continue;
+      ask(step + 2, stage == 0 ? 2 : stage - 1);
+      const unsigned char* here = smem + stage * plan.stage1;
+      stage = stage == 2 ? 0 : stage + 1;
+      if (j0 >= rank || kb0 + step * parts + part >= kb1 || r0 >= tile.rows) continue;
+      const uint2* x = reinterpret_cast<const uint2*>(here + part * kRows * 32) + (r0 + g) * 4 + t;
+      const float2* xs = reinterpret_cast<const float2*>(here + scales_at + part * kRows * 4 + r0 * 4) + t;
       const uint4* a = reinterpret_cast<const uint4*>(here + a_at) + ((size_t)(j0 + g) << row_log) + ((part * 4) ^ (g & 1 ? swap : 0)) + t;
-      uint4 r[2][2] = {};
+      uint4 c[4];
+      float2 sc[4];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        r[0][h] = a[(8 * h) << row_log];
-        if (two) r[1][h] = a[(16 + 8 * h) << row_log];
+      for (int i = 0; i < 4; ++i) {
+        c[i] = eight_of<kBf16>(x[i * 32]);
+        sc[i] = xs[i * 4];
       }
-      const uint2* x = reinterpret_cast<const uint2*>(here + part * kRows * 32) + g * 4 + t;
-      const float2* xs = reinterpret_cast<const float2*>(here + scales_at + part * kRows * 4) + t;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (i * 8 >= tile.rows) break;
-        const uint4 c = eight_of<kBf16>(x[i * 32]);
-        const float2 sc = xs[i * 4];
+      for (int m = 0; m < 4; ++m) {
+        if (j0 + 16 * m >= rank) break;
+        const uint4 a0 = a[(16 * m) << row_log], a1 = a[(16 * m + 8) << row_log];
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
+        for (int i = 0; i < 4; ++i) {
           float d[4] = {};
-          mma32<kBf16>(d, r[m][0], r[m][1], c);
-          acc[m][i][0] = fmaf(sc.x, d[0], acc[m][i][0]);
-          acc[m][i][1] = fmaf(sc.y, d[1], acc[m][i][1]);
-          acc[m][i][2] = fmaf(sc.x, d[2], acc[m][i][2]);
-          acc[m][i][3] = fmaf(sc.y, d[3], acc[m][i][3]);
+          mma32<kBf16>(d, a0, a1, c[i]);
+          acc[m][i][0] = fmaf(sc[i].x, d[0], acc[m][i][0]);
+          acc[m][i][1] = fmaf(sc[i].y, d[1], acc[m][i][1]);
+          acc[m][i][2] = fmaf(sc[i].x, d[2], acc[m][i][2]);
+          acc[m][i][3] = fmaf(sc[i].y, d[3], acc[m][i][3]);
         }
       }
     }
     copies_there<0>();
     __syncthreads();  // (the partial sums go over the stages)
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
+    for (int m = 0; m < 4; ++m)
       if (j0 + 16 * m < rank)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          float* to = s_part + ((size_t)part * p.R + j0 + 16 * m + g) * kRows + 8 * i + 2 * t;
+        for (int i = 0; i < 4; ++i) {
+          float* to = s_part + ((size_t)part * p.R + j0 + 16 * m + g) * kRows + r0 + 8 * i + 2 * t;
           *reinterpret_cast<float2*>(to) = make_float2(acc[m][i][0], acc[m][i][1]);
           *reinterpret_cast<float2*>(to + 8 * kRows) = make_float2(acc[m][i][2], acc[m][i][3]);
         }
@@ -528,6 +536,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_rows_kernel(LoraArgs p, Rows
   __syncthreads();
   cluster_wait();  // every CTA has begun
   // the CTA's sums, four rows per thread, to the CTA that joins these rows
+  const int own = kRows / p.cluster;  // (8, 16, 32 or 64)
   for (int i = tid; i < rank * (kRows / 4); i += kThreads) {
     const int j = i / (kRows / 4), row = i % (kRows / 4) * 4;
     float4 v = *reinterpret_cast<const float4*>(s_part + (size_t)j * kRows + row);
@@ -535,190 +544,252 @@ __global__ void __launch_bounds__(kThreads, 2) lora_rows_kernel(LoraArgs p, Rows
       const float4 b = *reinterpret_cast<const float4*>(s_part + ((size_t)w * p.R + j) * kRows + row);
       v.x += b.x; v.y += b.y; v.z += b.z; v.w += b.w;
     }
-    remote_store(at_rank(s_all + ((size_t)rank_of_cta * p.R + j) * kOwn + row % kOwn, row / kOwn), v);
+    remote_store(at_rank(s_all + ((size_t)rank_of_cta * p.R + j) * own + (row & (own - 1)), row / own), v);
   }
   cluster_arrive();
   cluster_wait();
+  // ---- a warp per row of its CTA: the sums of the CTAs in order
+  uint16_t* u = reinterpret_cast<uint16_t*>(scratch + plan.at_pieces + (size_t)index * plan.pieces);
+  float* factors = reinterpret_cast<float*>(scratch + plan.at_factors) + (size_t)index * kRows;
+  for (int i = warp; i < own; i += kWarps) {
+    const int row = rank_of_cta * own + i;
+    if (row >= tile.rows) {
+      for (int k = lane; k < kPieces<kBf16> * plan.ld; k += 32) u[(size_t)(k / plan.ld) * kRows * plan.ld + row * plan.ld + k % plan.ld] = 0;
+      if (lane == 0) factors[row] = 0.0f;
+      continue;
+    }
+    const float f = make_pieces<kBf16>(u + row * plan.ld, (size_t)kRows * plan.ld, rank, plan.ld, [&](int j) {
+      const float* from = s_all + (size_t)j * own + i;
+      float sum = 0.0f;
+#pragma unroll 8
+      for (int c = 0; c < p.cluster; ++c) sum += from[(size_t)c * p.R * own];
+      return sum;
+    }, (row & 1 ? plan.swap : 0) * 8);
+    if (lane == 0) factors[row] = tile.scale * f;
+  }
+}
 
-  // ---- steps of 64 outputs of the CTA's share: B's rows and the base come through stages, the first of them from here on
-  const int steps_all = (p.N + kCols - 1) / kCols, step0 = share(steps_all, kRowsCluster, rank_of_cta), steps = share(steps_all, kRowsCluster, rank_of_cta + 1) - step0;
+// The second product, base and outputs: steps of 64 rows x 64 outputs, an equal stretch of all of them for each CTA.
+// kRegs: the ranks are 64 at most, and a warp holds its rows' pieces in registers
+template <bool kBf16, bool kVec, bool kRegs>
+__global__ void __launch_bounds__(kThreads, 2) lora_outer_kernel(LoraArgs p, RowsPlan plan, const unsigned char* scratch) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3, ld = plan.ld;
   const int m0 = (warp & 3) * 16, half = (warp >> 2) * 32;  // a warp has 16 rows and 32 of the 64 outputs
-  const size_t row = tile.row + m0 + g;
-  const bool has0 = m0 + g < tile.rows, has1 = m0 + g + 8 < tile.rows;
-  const int b_row = tid >> 2, b_chunk = tid & 3, b_swap = b_row & 1 ? plan.swap : 0;  // four threads copy a row of B
-  const uint32_t b_to = stages_at + b_row * ld * 2 + b_chunk * 16, base_to = stages_at + kCols * ld * 2 + tid * 16;
-  const uint16_t* b_from = B + (size_t)(step0 * kCols + b_row) * p.R + b_chunk * 8;
-  const float* base_from = p.base ? p.base + row * p.ldb + step0 * kCols + half + 4 * t : nullptr;
-  const size_t eight = (size_t)8 * p.ldb;
-  auto ask = [&](int step, int stage) {
-    if (step < steps) {
-      const uint32_t at = stage * plan.stage2;
-      const int n0 = (step0 + step) * kCols;
-      const bool whole = n0 + kCols <= p.N;
-      const uint16_t* from = whole ? b_from + (size_t)step * kCols * p.R : B + (size_t)min(n0 + b_row, p.N - 1) * p.R + b_chunk * 8;
-      for (int c = 0; c * 8 < rank; c += 4)
-        if ((c + b_chunk) * 8 < rank) copy16(b_to + at + (c ^ b_swap) * 16, from + c * 8);
-      if (base_from) {  // each lane what it will add: rows g and g + 8, four outputs of both of its warp's sixteens
-        const float* of = base_from + (size_t)step * kCols;
-        if (kVec && whole) {
-          if (has0) {
-            copy16(base_to + at, of);
-            copy16(base_to + at + 2 * kThreads * 16, of + 16);
-          }
-          if (has1) {
-            copy16(base_to + at + kThreads * 16, of + eight);
-            copy16(base_to + at + 3 * kThreads * 16, of + eight + 16);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int n = n0 + half + (i >> 1) * 16 + 4 * t;
-            if (!(i & 1 ? has1 : has0)) continue;
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              if (n + k < p.N) copy4(base_to + at + i * kThreads * 16 + k * 4, of + (i & 1 ? eight : 0) + (i >> 1) * 16 + k);
-          }
-        }
-      }
-    }
-    copies_begun();
-  };
-  for (int i = 0; i < plan.stages2 - 1; ++i) ask(i, i);
+  const uint16_t* s_u = reinterpret_cast<const uint16_t*>(smem);
+  const uint32_t smem_at = (uint32_t)__cvta_generic_to_shared(smem), stages_at = smem_at + plan.pieces;
+  const bool in_place = p.base == p.C;
+  pdl_launch_next();
+  pdl_wait();
+  const int per = (p.N + kCols - 1) / kCols;
+  const long long all = (long long)*reinterpret_cast<const int*>(scratch) * per;
+  const long long begin = all * blockIdx.x / gridDim.x, end = all * (blockIdx.x + 1) / gridDim.x;
+  if (begin >= end) return;
+  const Tile* tiles = reinterpret_cast<const Tile*>(scratch + plan.at_tiles);
 
-  // ---- a warp per row of its CTA; the pieces go to every CTA
-  const int padded = ld;
   const size_t piece = (size_t)kRows * ld;
-  {
-    static_assert(kOwn == kWarps, "a warp per row");
-    const int own = rank_of_cta * kOwn + warp;
-    const float f = make_pieces<kBf16>(s_u + own * ld, piece, own < tile.rows ? rank : 0, padded, [&](int j) {
-      float u = s_all[(size_t)j * kOwn + warp];
-#pragma unroll
-      for (int c = 1; c < kRowsCluster; ++c) u += s_all[((size_t)c * p.R + j) * kOwn + warp];
-      return u;
-    }, (own & 1 ? plan.swap : 0) * 8);
-    __syncwarp();
-    for (int i = lane; i < kPieces<kBf16> * (padded / 8); i += 32) {
-      const uint16_t* here = s_u + (i / (padded / 8)) * piece + own * ld + i % (padded / 8) * 8;
-      const float4 v = *reinterpret_cast<const float4*>(here);
-      for (int c = 0; c < kRowsCluster; ++c)
-        if (c != rank_of_cta) remote_store(at_rank(here, c), v);
-    }
-    if (lane < kRowsCluster) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at_rank(&s_factor[own], lane)), "f"(f) : "memory");
-  }
-  cluster_arrive();
-  cluster_wait();
-
-  // ---- outputs
-  const float f0 = tile.scale * s_factor[m0 + g], f1 = tile.scale * s_factor[m0 + g + 8];
-  float *c0 = p.C + row * p.ldc + step0 * kCols + half + 4 * t, *c1 = c0 + 8 * (size_t)p.ldc;
   const int col = 4 * (g >> 1) + (g & 1);     // column g of the first instruction; of the second one: two further
   const int swap = g & 1 ? plan.swap : 0;     // (rows g + 8, columns two further: as odd as g)
   const uint16_t *u0 = s_u + (m0 + g) * ld + t * 8, *u1 = u0 + 8 * ld;
-  uint4 held[kRegs ? 2 : 1][kPieces<kBf16>][2];
-  if (kRegs) {
+  const int b_row = tid >> 2, b_chunk = tid & 3;  // four threads copy a row of B
+  const uint32_t b_to = stages_at + (b_row * ld + (b_chunk ^ (b_row & 1 ? plan.swap : 0)) * 8) * 2, b_swap = b_row & 1 && plan.swap ? 0xFFFFFFC0u : 64u;  // (the next four chunks)
+  const uint32_t base_to = stages_at + kCols * ld * 2 + tid * 16;
+  uint4 held[kRegs ? 2 : 1][kPieces<kBf16>][2] = {};
+
+  // A tile's steps in this CTA's stretch, one tile after the other
+  int index = (int)(begin / per), step0 = (int)(begin % per);
+  for (long long left = end - begin; left > 0; ++index, step0 = 0) {
+    const Tile tile = tiles[index];
+    const int steps = (int)min(left, (long long)(per - step0)), rank = (tile.rank + 15) & ~15;
+    left -= steps;
+    if (in_place && rank == 0) continue;
+    __syncthreads();  // (everybody has done with the tile before)
+
+    // ---- copies: a row of B per four threads, and for each lane what it will add: rows g and g + 8, four outputs of both of its warp's sixteens
+    const int mine = (rank / 8 - b_chunk + 3) / 4;  // 16-byte chunks of the row for this thread
+    const bool has0 = m0 + g < tile.rows, has1 = m0 + g + 8 < tile.rows;
+    const uint16_t* b_from = p.B + ((size_t)(rank ? tile.adapter : 0) * p.N + step0 * kCols + b_row) * p.R + b_chunk * 8;
+    const size_t row = tile.row + m0 + g;
+    // (rows past the tile's: the last one again, which nobody stores)
+    const float* from0 = p.base + (size_t)(tile.row + min(m0 + g, tile.rows - 1)) * p.ldb + step0 * kCols + half + 4 * t;
+    const float* from1 = p.base + (size_t)(tile.row + min(m0 + g + 8, tile.rows - 1)) * p.ldb + step0 * kCols + half + 4 * t;
+    int ask_n = step0 * kCols;         // the next step's first output
+    int ask_left = steps;
+    uint32_t ask_at = 0;               // its stage
+    const uint32_t stages_end = plan.stages2 * plan.stage2;
+    auto ask = [&]() {
+      if (ask_left > 0) {
+        --ask_left;
+        if (ask_n + kCols <= p.N) {
+          if (kRegs) {
+            if (mine > 0) copy16(b_to + ask_at, b_from);
+            if (mine > 1) copy16(b_to + ask_at + b_swap, b_from + 32);
+          } else {
+            for (int c = 0; c < mine; ++c) copy16(b_to + ask_at + (c >> 1) * 128 + (c & 1 ? b_swap : 0u), b_from + 32 * c);
+          }
+        } else {
+          const uint16_t* from = p.B + ((size_t)(rank ? tile.adapter : 0) * p.N + min(ask_n + b_row, p.N - 1)) * p.R + b_chunk * 8;
+          for (int c = 0; c < mine; ++c) copy16(b_to + ask_at + (c >> 1) * 128 + (c & 1 ? b_swap : 0u), from + 32 * c);
+        }
+        b_from += (size_t)kCols * p.R;
+        if (p.base) {
+          const uint32_t to = base_to + ask_at;
+          if (kVec && ask_n + kCols <= p.N) {
+            copy16(to, from0);
+            copy16(to + kThreads * 16, from1);
+            copy16(to + 2 * kThreads * 16, from0 + 16);
+            copy16(to + 3 * kThreads * 16, from1 + 16);
+          } else {
+            const int n = ask_n + half + 4 * t;
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int k = 0; k < kPieces<kBf16>; ++k) {
-        held[kRegs ? j : 0][k][0] = 32 * j < ld ? *reinterpret_cast<const uint4*>(u0 + k * piece + (4 * j ^ swap) * 8) : make_uint4(0u, 0u, 0u, 0u);
-        held[kRegs ? j : 0][k][1] = 32 * j < ld ? *reinterpret_cast<const uint4*>(u1 + k * piece + (4 * j ^ swap) * 8) : make_uint4(0u, 0u, 0u, 0u);
+            for (int k = 0; k < 4; ++k) {
+              if (n + k < p.N) {
+                copy4(to + k * 4, from0 + k);
+                copy4(to + kThreads * 16 + k * 4, from1 + k);
+              }
+              if (n + 16 + k < p.N) {
+                copy4(to + 2 * kThreads * 16 + k * 4, from0 + 16 + k);
+                copy4(to + 3 * kThreads * 16 + k * 4, from1 + 16 + k);
+              }
+            }
+          }
+          from0 += kCols;
+          from1 += kCols;
+        }
+        ask_n += kCols;
+        ask_at += plan.stage2;
+        if (ask_at == stages_end) ask_at = 0;
       }
-  }
-  for (int step = 0, stage = 0; step < steps; ++step) {
-    copies_there(plan.stages2 - 2);
-    __syncthreads();  // this stage has arrived for everybody, and everybody has done with the one before
-    ask(step + plan.stages2 - 1, stage == 0 ? plan.stages2 - 1 : stage - 1);
-    const unsigned char* here = smem + plan.first + stage * plan.stage2;
-    stage = stage + 1 == plan.stages2 ? 0 : stage + 1;
-    if (m0 >= tile.rows) continue;
-    const uint16_t* b = reinterpret_cast<const uint16_t*>(here) + (half + col) * ld + t * 8;
-    float d[2][2][4] = {};
-    // 32 ranks of a tile: sixteen columns h, instruction i
-    auto of_b = [&](int h, int i, int chunk) { return b + (16 * h + 2 * i) * ld + (chunk ^ swap) * 8; };
-    if (kRegs) {
-      // (B's columns between the adapter's rank and a multiple of 32 are what was there before: zeros by the pieces only if they are numbers, so sixteens
-      // are taken by themselves)
+      copies_begun();
+    };
+    for (int i = 0; i < plan.stages2 - 1; ++i) ask();
+
+    // ---- u's pieces
+    float f0 = 0.0f, f1 = 0.0f;
+    if (rank) {
+      const uint4* from = reinterpret_cast<const uint4*>(scratch + plan.at_pieces + (size_t)index * plan.pieces);
+      for (uint32_t k = tid; k < plan.pieces / 16; k += kThreads) reinterpret_cast<uint4*>(smem)[k] = from[k];
+      const float* factors = reinterpret_cast<const float*>(scratch + plan.at_factors) + (size_t)index * kRows + m0 + g;
+      f0 = factors[0];
+      f1 = factors[8];
+      __syncthreads();
+      if (kRegs) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        if (32 * j + 32 <= rank) {
+        for (int j = 0; j < 2; ++j)
+          if (32 * j < ld)
+#pragma unroll
+            for (int k = 0; k < kPieces<kBf16>; ++k) {
+              held[kRegs ? j : 0][k][0] = *reinterpret_cast<const uint4*>(u0 + k * piece + (4 * j ^ swap) * 8);
+              held[kRegs ? j : 0][k][1] = *reinterpret_cast<const uint4*>(u1 + k * piece + (4 * j ^ swap) * 8);
+            }
+      }
+    }
+
+    // ---- outputs
+    const unsigned char* here = smem + plan.pieces;
+    float *c0 = p.C + row * p.ldc + step0 * kCols + half + 4 * t, *c1 = c0 + 8 * (size_t)p.ldc;
+    int n = step0 * kCols + half + 4 * t;
+    for (int i = 0; i < steps; ++i, n += kCols, c0 += kCols, c1 += kCols) {
+      copies_there(plan.stages2 - 2);
+      __syncthreads();  // this stage has arrived for everybody, and everybody has done with the one before
+      ask();
+      const uint16_t* b = reinterpret_cast<const uint16_t*>(here) + (half + col) * ld + t * 8;
+      const float4* old = reinterpret_cast<const float4*>(here + kCols * ld * 2) + tid;
+      here += plan.stage2;
+      if (here == smem + plan.pieces + stages_end) here = smem + plan.pieces;
+      if (m0 >= tile.rows) continue;
+      float d[2][2][4] = {};
+      // chunks of 32 ranks of B's rows: sixteen outputs h, instruction q
+      auto of_b = [&](int h, int q, int chunk) { return b + (16 * h + 2 * q) * ld + (chunk ^ swap) * 8; };
+      if (kRegs) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          if (32 * j + 32 <= rank) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int q = 0; q < 2; ++q) {
+                const uint4 v = *reinterpret_cast<const uint4*>(of_b(h, q, 4 * j));
+#pragma unroll
+                for (int k = 0; k < kPieces<kBf16>; ++k) mma32<kBf16>(d[h][q], held[kRegs ? j : 0][k][0], held[kRegs ? j : 0][k][1], v);
+              }
+          }
+        }
+      }
+      int j = kRegs ? rank & ~31 : 0;
+      if (!kRegs)
+        for (; j + 32 <= rank; j += 32) {
+          uint4 v[2][2];
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const uint4 v = *reinterpret_cast<const uint4*>(of_b(h, i, 4 * j));
+            for (int q = 0; q < 2; ++q) v[h][q] = *reinterpret_cast<const uint4*>(of_b(h, q, j / 8));
 #pragma unroll
-              for (int k = 0; k < kPieces<kBf16>; ++k) mma32<kBf16>(d[h][i], held[kRegs ? j : 0][k][0], held[kRegs ? j : 0][k][1], v);
+          for (int k = 0; k < kPieces<kBf16>; ++k) {
+            const uint4 r0 = *reinterpret_cast<const uint4*>(u0 + k * piece + (j / 8 ^ swap) * 8), r1 = *reinterpret_cast<const uint4*>(u1 + k * piece + (j / 8 ^ swap) * 8);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int q = 0; q < 2; ++q) mma32<kBf16>(d[h][q], r0, r1, v[h][q]);
+          }
+        }
+      if (j < rank) {  // sixteen more: a lane has four of them, in chunk t / 2 of the two
+        const int at = (j / 8 ^ swap) * 8 + 4 * t - 8 * t;
+#pragma unroll
+        for (int k = 0; k < kPieces<kBf16>; ++k) {
+          const uint2 r0 = *reinterpret_cast<const uint2*>(u0 + k * piece + at), r1 = *reinterpret_cast<const uint2*>(u1 + k * piece + at);
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              const uint2 v = *reinterpret_cast<const uint2*>(b + (16 * h + 2 * q) * ld + at);
+              mma<kBf16>(d[h][q], r0.x, r1.x, r0.y, r1.y, v.x, v.y);
+            }
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float4 o0 = make_float4(0.0f, 0.0f, 0.0f, 0.0f), o1 = o0;
+        if (p.base) {
+          o0 = old[2 * h * kThreads];
+          o1 = old[(2 * h + 1) * kThreads];
+        }
+        if (rank) {
+          o0 = make_float4(fmaf(f0, d[h][0][0], o0.x), fmaf(f0, d[h][0][1], o0.y), fmaf(f0, d[h][1][0], o0.z), fmaf(f0, d[h][1][1], o0.w));
+          o1 = make_float4(fmaf(f1, d[h][0][2], o1.x), fmaf(f1, d[h][0][3], o1.y), fmaf(f1, d[h][1][2], o1.z), fmaf(f1, d[h][1][3], o1.w));
+        }
+        if (kVec && n - half - 4 * t + kCols <= p.N) {
+          if (has0) *reinterpret_cast<float4*>(c0 + 16 * h) = o0;
+          if (has1) *reinterpret_cast<float4*>(c1 + 16 * h) = o1;
+        } else {
+          const float v0[4] = {o0.x, o0.y, o0.z, o0.w}, v1[4] = {o1.x, o1.y, o1.z, o1.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (n + 16 * h + k < p.N) {
+              if (has0) c0[16 * h + k] = v0[k];
+              if (has1) c1[16 * h + k] = v1[k];
             }
         }
       }
     }
-    int j = kRegs ? rank & ~31 : 0;
-    for (; j + 32 <= rank; j += 32) {
-      uint4 v[2][2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) v[h][i] = *reinterpret_cast<const uint4*>(of_b(h, i, j / 8));
-#pragma unroll
-      for (int k = 0; k < kPieces<kBf16>; ++k) {
-        const uint4 r0 = *reinterpret_cast<const uint4*>(u0 + k * piece + (j / 8 ^ swap) * 8), r1 = *reinterpret_cast<const uint4*>(u1 + k * piece + (j / 8 ^ swap) * 8);
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) mma32<kBf16>(d[h][i], r0, r1, v[h][i]);
-      }
-    }
-    if (j < rank) {  // sixteen more: a lane has four of them, in chunk t / 2 of the two
-      const int at = (j / 8 ^ swap) * 8 + 4 * t - 8 * t;
-#pragma unroll
-      for (int k = 0; k < kPieces<kBf16>; ++k) {
-        const uint2 r0 = *reinterpret_cast<const uint2*>(u0 + k * piece + at), r1 = *reinterpret_cast<const uint2*>(u1 + k * piece + at);
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint2 v = *reinterpret_cast<const uint2*>(b + (16 * h + 2 * i) * ld + at);
-            mma<kBf16>(d[h][i], r0.x, r1.x, r0.y, r1.y, v.x, v.y);
-          }
-      }
-    }
-    const float4* old = reinterpret_cast<const float4*>(here + kCols * ld * 2) + tid;
-    const int n = (step0 + step) * kCols + half + 4 * t;
-    const bool whole = (step0 + step + 1) * kCols <= p.N;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float4 o0 = make_float4(0.0f, 0.0f, 0.0f, 0.0f), o1 = o0;
-      if (p.base) {
-        o0 = old[2 * h * kThreads];
-        o1 = old[(2 * h + 1) * kThreads];
-      }
-      o0 = make_float4(fmaf(f0, d[h][0][0], o0.x), fmaf(f0, d[h][0][1], o0.y), fmaf(f0, d[h][1][0], o0.z), fmaf(f0, d[h][1][1], o0.w));
-      o1 = make_float4(fmaf(f1, d[h][0][2], o1.x), fmaf(f1, d[h][0][3], o1.y), fmaf(f1, d[h][1][2], o1.z), fmaf(f1, d[h][1][3], o1.w));
-      if (kVec && whole) {
-        if (has0) *reinterpret_cast<float4*>(c0 + 16 * h) = o0;
-        if (has1) *reinterpret_cast<float4*>(c1 + 16 * h) = o1;
-      } else {
-        const float v0[4] = {o0.x, o0.y, o0.z, o0.w}, v1[4] = {o1.x, o1.y, o1.z, o1.w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (n + 16 * h + k < p.N) {
-            if (has0) c0[16 * h + k] = v0[k];
-            if (has1) c1[16 * h + k] = v1[k];
-          }
-      }
-    }
-    c0 += kCols;
-    c1 += kCols;
+    copies_there<0>();
   }
-  copies_there<0>();
 }
+
+constexpr int kMaxInner = 200 << 10;
+bool few_rows(int T, int n_seg) { return T <= 8 * (int64_t)n_seg; }
 
 }  // namespace
 
+extern "C" size_t izb_lora_scratch(int dtype, int R, int T, int n_seg) {
+  if (T < 1 || n_seg < 1 || R < 16 || R > kMaxRank || few_rows(T, n_seg)) return 0;
+  const size_t tiles = (size_t)T / kRows + n_seg;
+  return RowsPlan(R, dtype == IZB_BF16, tiles).scratch(tiles);
+}
+
 extern "C" int izb_lora_add(int dtype, const void* d_A, const void* d_B, int n_adapters, int R, const int32_t* d_ranks, const float* d_scales, int N, int K,
                             const int8_t* d_aq, const float* d_asc, int T, int Mp, const int32_t* d_seg, const int32_t* d_adapter, int n_seg,
-                            const float* d_base, int ldb, float* d_C, int ldc, int c_off, void* stream) {
+                            const float* d_base, int ldb, float* d_C, int ldc, int c_off, void* d_scratch, void* stream) {
   if (!d_A || !d_B || !d_scales || !d_aq || !d_asc || !d_seg || !d_adapter || !d_C) IZB_FAIL(IZB_ERR_ARG, "lora_add: null pointer");
   if (dtype != IZB_F16 && dtype != IZB_BF16) IZB_FAIL(IZB_ERR_TYPE, "lora_add: adapters of type %d are not taken (IZB_F16, IZB_BF16)", dtype);
   if (n_adapters < 1 || R < 16 || R > kMaxRank || R % 16) IZB_FAIL(IZB_ERR_SHAPE, "lora_add: %d adapters of rank %d (16..%d, a multiple of 16: pad with zeros)", n_adapters, R, kMaxRank);
@@ -733,9 +804,12 @@ extern "C" int izb_lora_add(int dtype, const void* d_A, const void* d_B, int n_a
   IZB_CUDA(cudaGetDevice(&device));
   LoraArgs p = {(const uint16_t*)d_A, (const uint16_t*)d_B, d_ranks, d_seg, d_adapter, d_scales, d_asc, d_base, d_aq, d_C + c_off, n_adapters, R, N, K, T, Mp, n_seg, ldb, ldc, 0};
   cudaStream_t st = (cudaStream_t)stream;
-  const bool bf16 = dtype == IZB_BF16, few = T <= 8 * (int64_t)n_seg;
+  const bool bf16 = dtype == IZB_BF16, few = few_rows(T, n_seg);
   const int64_t tiles = (int64_t)T / (few ? kFewRows : kRows) + n_seg;  // (at most)
-  p.cluster = !few ? kRowsCluster : tiles * 16 <= 2 * izb_sm_count(device) && R <= 128 ? 16 : 8;
+  const int sms = izb_sm_count(device);
+  // CTAs per tile.  Few rows: 16 while that leaves the multiprocessors two CTAs at most, else 8.  More rows: as many as fit at once, 8 at most.
+  p.cluster = few && tiles * 16 <= 2 * sms && R <= 128 ? 16 : 8;
+  while (!few && p.cluster > 1 && tiles * p.cluster > 2 * sms) p.cluster /= 2;
   if (tiles * p.cluster > 0x7FFFFFFF) IZB_FAIL(IZB_ERR_LIMIT, "lora_add: %d rows in %d segments", T, n_seg);
   const dim3 grid((unsigned)(tiles * p.cluster));
   if (few) {
@@ -752,17 +826,29 @@ extern "C" int izb_lora_add(int dtype, const void* d_A, const void* d_B, int n_a
     IZB_LAUNCH("lora_add", st, izb_launch_pdl_cluster(bf16 ? lora_few_kernel<true> : lora_few_kernel<false>, p.cluster, grid, kThreads, smem, st, p));
     return IZB_OK;
   }
+  if (!d_scratch || !izb_aligned(d_scratch, 16)) IZB_FAIL(IZB_ERR_ARG, "lora_add: %d rows in %d segments want %zu bytes of scratch, 16-byte aligned", T, n_seg, izb_lora_scratch(dtype, R, T, n_seg));
+  const RowsPlan plan(R, bf16, tiles);
+  if (plan.scratch(tiles) > 0xFFFFFFFFu) IZB_FAIL(IZB_ERR_LIMIT, "lora_add: %d rows in %d segments of rank %d", T, n_seg, R);
   const bool vec = izb_aligned(p.C, 16) && ldc % 4 == 0 && (!d_base || (izb_aligned(d_base, 16) && ldb % 4 == 0));
-  static izb_device_once once[8];
-  void (*const kernels[8])(LoraArgs, RowsPlan) = {lora_rows_kernel<false, false, false>, lora_rows_kernel<false, false, true>, lora_rows_kernel<false, true, false>, lora_rows_kernel<false, true, true>,
-                                                  lora_rows_kernel<true, false, false>, lora_rows_kernel<true, false, true>, lora_rows_kernel<true, true, false>, lora_rows_kernel<true, true, true>};
+  static izb_device_once once[10];
+  void (*const inner)(LoraArgs, RowsPlan, unsigned char*) = bf16 ? lora_inner_kernel<true> : lora_inner_kernel<false>;
+  void (*const outers[8])(LoraArgs, RowsPlan, const unsigned char*) = {lora_outer_kernel<false, false, false>, lora_outer_kernel<false, false, true>, lora_outer_kernel<false, true, false>,
+                                                                       lora_outer_kernel<false, true, true>, lora_outer_kernel<true, false, false>, lora_outer_kernel<true, false, true>,
+                                                                       lora_outer_kernel<true, true, false>, lora_outer_kernel<true, true, true>};
   const int which = (bf16 ? 4 : 0) + (vec ? 2 : 0) + (R <= 64 ? 1 : 0);
   if (int rc = once[which].run(device, [&]() -> int {
-        IZB_CUDA(cudaFuncSetAttribute(kernels[which], cudaFuncAttributeMaxDynamicSharedMemorySize, (int)RowsPlan(R <= 64 ? 64 : kMaxRank, true).total));
+        IZB_CUDA(cudaFuncSetAttribute(outers[which], cudaFuncAttributeMaxDynamicSharedMemorySize, (int)RowsPlan(R <= 64 ? 64 : kMaxRank, true, 0).total2));
         return IZB_OK;
       }))
     return rc;
-  const RowsPlan plan(R, bf16);
-  IZB_LAUNCH("lora_add", st, izb_launch_pdl_cluster(kernels[which], kRowsCluster, grid, kThreads, plan.total, st, p, plan));
+  if (int rc = once[8 + bf16].run(device, [&]() -> int {
+        IZB_CUDA(cudaFuncSetAttribute(inner, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxInner));
+        return IZB_OK;
+      }))
+    return rc;
+  IZB_LAUNCH("lora_inner", st, izb_launch_pdl_cluster(inner, p.cluster, grid, kThreads, plan.total1, st, p, plan, (unsigned char*)d_scratch));
+  // (two CTAs per multiprocessor; no more than there is work at most)
+  const int64_t steps = tiles * ((N + kCols - 1) / kCols), outer_grid = steps < 2 * sms ? steps : 2 * sms;
+  IZB_LAUNCH("lora_outer", st, izb_launch_pdl(outers[which], dim3((unsigned)outer_grid), kThreads, plan.total2, st, p, plan, (const unsigned char*)d_scratch));
   return IZB_OK;
 }

@@ -23,7 +23,7 @@ namespace {
 #define IZB_PY_CALLS(X) \
   X(izb_quantize_act) X(izb_swiglu_quant) X(izb_rmsnorm_quant) X(izb_add_norm_quant) X(izb_softcap_rows) X(izb_matmul) X(izb_quant_matmul) \
   X(izb_gemv) X(izb_gemm) X(izb_moe_route_ex) X(izb_moe_sort_ex) X(izb_moe_gateup) X(izb_moe_down) X(izb_moe_combine_ex) \
-  X(izb_moe_layer) X(izb_moe_layer_scratch) X(izb_lora_add) X(izb_logits_process)
+  X(izb_moe_layer) X(izb_moe_layer_scratch) X(izb_lora_add) X(izb_lora_scratch) X(izb_logits_process)
 
 struct Calls {
 #define X(name) decltype(&name) name##_ = nullptr;
@@ -473,8 +473,13 @@ FN(lora_add) {
     base = static_cast<const float*>(b.data_ptr());
   }
   if (a[11] != Py_None) TORCH_CHECK_VALUE(whole(a[11], "ranks", {at::kInt}, 1).size(0) == n_ad, "ranks: one per adapter expected");
-  call(g.izb_lora_add_, A.scalar_type() == at::kHalf ? IZB_F16 : IZB_BF16, (const void*)A.data_ptr(), (const void*)B.data_ptr(), n_ad, R, ptr<int32_t>(a[11]), ptr<float>(a[2]), N, K,
-       ptr<int8_t>(a[3]), ptr<float>(a[4]), T, extent(a[4], 1), ptr<int32_t>(a[6]), ptr<int32_t>(a[7]), n_seg, base, ldb, static_cast<float*>(C.data_ptr()), ldc, c_off);
+  const int dtype = A.scalar_type() == at::kHalf ? IZB_F16 : IZB_BF16;
+  at::Tensor scratch;
+  const size_t bytes = g.izb_lora_scratch_(dtype, R, T, n_seg);
+  if (bytes) scratch = empty({(int64_t)bytes}, at::kByte, A.device());
+  call(g.izb_lora_add_, dtype, (const void*)A.data_ptr(), (const void*)B.data_ptr(), n_ad, R, ptr<int32_t>(a[11]), ptr<float>(a[2]), N, K,
+       ptr<int8_t>(a[3]), ptr<float>(a[4]), T, extent(a[4], 1), ptr<int32_t>(a[6]), ptr<int32_t>(a[7]), n_seg, base, ldb, static_cast<float*>(C.data_ptr()), ldc, c_off,
+       bytes ? scratch.data_ptr() : nullptr);
   return own(a[8]);
   END_HANDLE_TH_ERRORS
 }

@@ -153,9 +153,11 @@ class Engine {
     const int32_t* ranks = nullptr;
     const float* scales = nullptr;
   };
-  void lora_add(const Adapters& l, const int32_t* seg, const int32_t* adapter, int n_seg, float* C, int ldc, int c_off) {
+  size_t lora_scratch(const Adapters& l, int n_seg) const { return izb_lora_scratch(l.dtype, l.R, cur_T_, n_seg); }
+  void lora_add(const Adapters& l, const int32_t* seg, const int32_t* adapter, int n_seg, float* C, int ldc, int c_off, void* scratch) {
     if (l.K != cur_K_) throw std::runtime_error("lora_add: the quantised activations do not match these adapters");
-    check(izb_lora_add(l.dtype, l.A, l.B, l.n, l.R, l.ranks, l.scales, l.N, l.K, aq_, asc_, cur_T_, cur_Mp_, seg, adapter, n_seg, C + c_off, ldc, C, ldc, c_off, stream_),
+    check(izb_lora_add(l.dtype, l.A, l.B, l.n, l.R, l.ranks, l.scales, l.N, l.K, aq_, asc_, cur_T_, cur_Mp_, seg, adapter, n_seg, C + c_off, ldc, C, ldc, c_off, scratch,
+                       stream_),
           "lora_add");
   }
   // the expert block of a decode step's rows (izb_moe_layer): x [cur_T][E] += the experts' weighted sum over the quantised activations; scratch

@@ -249,10 +249,13 @@ int izb_gemm(const izb_weight* w, int mat, const int8_t* d_aq, const float* d_as
  * to it.  d_seg [n_seg + 1]: row offsets, increasing (equal ones: an empty segment); what lies outside 0..T is cut off.  Rows before d_seg[0]
  * and behind the last segment are left as they were.  base: d_base [T][ldb] (its first column), d_base = d_C + c_off with ldb = ldc to add in place, or
  * NULL for zeros; rows of segments without an adapter receive the base.  Sums in f32 in an order that depends on the row's place in its segment's
- * tiles alone, not on other rows.  A, B, aq, asc 16-byte aligned, base and C any f32 address (16-byte aligned rows are faster). */
+ * tiles and the call's number of rows and segments alone, not on other rows' values.  A row whose inner sums are no finite numbers is NaN.
+ * A, B, aq, asc 16-byte aligned, base and C any f32 address (16-byte aligned rows are faster).  d_scratch: izb_lora_scratch(dtype, R, T, n_seg) bytes (0 for
+ * up to 8 rows per segment on average: then NULL will do), 16-byte aligned, the call's own until it has finished. */
+size_t izb_lora_scratch(int dtype, int R, int T, int n_seg);
 int izb_lora_add(int dtype, const void* d_A, const void* d_B, int n_adapters, int R, const int32_t* d_ranks, const float* d_scales, int N, int K,
                  const int8_t* d_aq, const float* d_asc, int T, int Mp, const int32_t* d_seg, const int32_t* d_adapter, int n_seg, const float* d_base,
-                 int ldb, float* d_C, int ldc, int c_off, void* stream);
+                 int ldb, float* d_C, int ldc, int c_off, void* d_scratch, void* stream);
 /* Verification mode (the reference's xmx_check idea, zero/engine_setup.h:424): the per-32-block integer dot products
  * themselves, d_dots int32 [M][N][K/32], from the CUDA-core kernel (impl = IZB_GEMM_CORE) or from the tensor-core
  * kernel's accumulators before any scaling (impl = IZB_GEMM_TC).  Both must equal the CPU values bit for bit. */

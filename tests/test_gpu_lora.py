@@ -102,7 +102,9 @@ def test_without_a_base(izb, torch):
     c = Case(izb, torch, [3, 2, 70], [1, -1, 0], [16, 16], 100, 512, "f16")
     out = torch.full((c.T, 100), float("nan"), device="cuda")
     q = lambda t: C.c_void_p(t.data_ptr())
-    rc = izb.lib().izb_lora_add(1, q(c.A), q(c.B), 2, 16, None, q(c.scales), 100, 512, q(c.aq), q(c.asc), c.T, c.asc.shape[1], q(c.seg), q(c.adapter), 3, None, 0, q(out), 100, 0,
+    izb.lib().izb_lora_scratch.restype = C.c_size_t
+    scratch = torch.empty(izb.lib().izb_lora_scratch(1, 16, c.T, 3), dtype=torch.uint8, device="cuda")
+    rc = izb.lib().izb_lora_add(1, q(c.A), q(c.B), 2, 16, None, q(c.scales), 100, 512, q(c.aq), q(c.asc), c.T, c.asc.shape[1], q(c.seg), q(c.adapter), 3, None, 0, q(out), 100, 0, q(scratch),
                                 C.c_void_p(torch.cuda.current_stream().cuda_stream))
     assert rc == 0
     want, room = c.want(torch.zeros_like(c.base))

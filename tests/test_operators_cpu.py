@@ -23,7 +23,7 @@ def aligned(n, dtype=np.float32):
 def lora(**kw):
     b = aligned(65536)
     a = dict(dtype=1, A=p(b), B=p(b), n=2, R=16, ranks=None, scales=p(b), N=32, K=256, aq=p(b), asc=p(b), T=3, Mp=16, seg=p(b), adapter=p(b), n_seg=1, base=None, ldb=32,
-             C=p(b), ldc=32, c_off=0)
+             C=p(b), ldc=32, c_off=0, scratch=None)
     a.update(kw)
     return izb.lib().izb_lora_add(*a.values(), None)
 
