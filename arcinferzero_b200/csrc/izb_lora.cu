@@ -96,11 +96,23 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// 32 elements of the inner dimension: a lane holds elements 8t .. 8t+7 of its row on either side (two instructions' worth)
+// 32 elements of the inner dimension in two instructions.  The order of the elements within the 32 is free: a lane's elements are 8t .. 8t+7, its column's as
+// they lie in memory (16 bytes).  `lo`, `hi`: the row side's registers of the two instructions -- rows g and g + 8 alternate in them, which is why that side
+// is always one that is made in registers or laid out for it, and the adapters are the column side: rows as they come would have to be moved together.
 template <bool kBf16>
-__device__ __forceinline__ void mma32(float (&d)[4], uint4 r0, uint4 r1, uint4 c) {
-  mma<kBf16>(d, r0.x, r1.x, r0.y, r1.y, c.x, c.y);
-  mma<kBf16>(d, r0.z, r1.z, r0.w, r1.w, c.z, c.w);
+__device__ __forceinline__ void mma32(float (&d)[4], uint4 lo, uint4 hi, uint4 c) {
+  mma<kBf16>(d, lo.x, lo.y, lo.z, lo.w, c.x, c.y);
+  mma<kBf16>(d, hi.x, hi.y, hi.z, hi.w, c.z, c.w);
+}
+// Where element j of a row of `rank` is among such registers: the 16 bytes of a lane, as a number of 32-lane groups, and the 16-bit value in them.  (The last
+// sixteen of a rank that is no multiple of 32 are one instruction's, four per lane.)
+struct Place {
+  int group, t, value;  // (value: 4 * register pair + half)
+};
+__device__ __forceinline__ Place place_of(int j, int rank) {
+  const int chunk = j >> 5;
+  if (chunk * 32 + 32 <= rank) return {chunk * 2 + ((j >> 2) & 1), (j & 31) >> 3, ((j >> 1) & 1) * 4 + (j & 1)};
+  return {chunk * 2, (j & 15) >> 2, ((j >> 1) & 1) * 4 + (j & 1)};
 }
 // Two int8 values (bytes i, i + 1) as 16-bit floats.  f16: the byte with its sign bit flipped is v + 128, and under the exponent of 1024 it is 1152 + v.
 // bf16 has seven bits of fraction: the byte without its sign bit under the exponent of 128, less 128 -- or 256 where the sign bit is set.
@@ -123,18 +135,18 @@ __device__ __forceinline__ uint4 eight_of(uint2 v) {
 
 template <bool kBf16>
 constexpr int kPieces = kBf16 ? 3 : 2;
-// A warp makes the pieces of a row from its sums; the factor that the second product's result takes.  A row with a sum that is no finite number is NaN.
-// `swap`: what the places' numbers are xored with.
-template <bool kBf16, class Sum>
-__device__ __forceinline__ float make_pieces(uint16_t* to, size_t piece_stride, int rank, int padded, Sum sum, int swap = 0) {
+// A warp makes the pieces of a row from its sums, put(piece, j, 16-bit value); the factor that the second product's result takes.  A row with a sum that is no
+// finite number is NaN.
+template <bool kBf16, class Sum, class Put>
+__device__ __forceinline__ float make_pieces(int rank, Sum sum, Put put) {
   const int lane = threadIdx.x & 31;
   if (kBf16) {
-    for (int j = lane; j < padded; j += 32) {
-      float u = j < rank ? sum(j) : 0.0f;
+    for (int j = lane; j < rank; j += 32) {
+      float u = sum(j);
 #pragma unroll
       for (int i = 0; i < 3; ++i) {
         const __nv_bfloat16 h = __float2bfloat16_rn(u);
-        to[i * piece_stride + (j ^ swap)] = __bfloat16_as_ushort(h);
+        put(i, j, __bfloat16_as_ushort(h));
         u -= __bfloat162float(h);
       }
     }
@@ -145,7 +157,8 @@ __device__ __forceinline__ float make_pieces(uint16_t* to, size_t piece_stride, 
 #pragma unroll
   for (int i = 0; i < kMaxRank / 32; ++i) {
     const int j = i * 32 + lane;
-    u[i] = j < rank ? sum(j) : 0.0f;
+    u[i] = 0.0f;
+    if (i * 32 < rank && j < rank) u[i] = sum(j);
     most = max(most, __float_as_uint(u[i]) & 0x7FFFFFFFu);
   }
   most = __reduce_max_sync(0xFFFFFFFFu, most);
@@ -154,11 +167,11 @@ __device__ __forceinline__ float make_pieces(uint16_t* to, size_t piece_stride, 
 #pragma unroll
   for (int i = 0; i < kMaxRank / 32; ++i) {
     const int j = i * 32 + lane;
-    if (j >= padded) break;
+    if (i * 32 >= rank || j >= rank) break;
     const float v = none ? __uint_as_float(0x7FC00000u) : ldexpf(u[i], 13 - ex);
     const __half h = __float2half_rn(v);
-    to[j ^ swap] = __half_as_ushort(h);
-    to[piece_stride + (j ^ swap)] = __half_as_ushort(__float2half_rn(v - __half2float(h)));
+    put(0, j, __half_as_ushort(h));
+    put(1, j, __half_as_ushort(__float2half_rn(v - __half2float(h))));
   }
   return ldexpf(1.0f, ex - 13);
 }
@@ -190,21 +203,23 @@ __device__ __forceinline__ void copy_base(const LoraArgs& p, const Tile& tile, i
 constexpr int kFewRows = 8;
 constexpr int kFewRanks = 4;   // rank tiles of 16 at a time
 constexpr int kFewSlots = 8;   // pieces of an adapter (16 rows x 32 elements, 1 KB) that a warp has asked for: 64 KB per CTA
+constexpr int kFewPart = kFewRanks * 16 + 8;  // a row of partial sums (the padding: rows on different banks)
+// rings | partial sums of the warps | those of the CTAs | the pieces of u, two to an instruction
 static size_t few_smem(int R, int cluster) {
-  // rings | partial sums of the warps | those of the CTAs | the pieces of u (three at most)
-  return (size_t)kWarps * kFewSlots * 1024 + (size_t)kWarps * kFewRanks * 16 * 8 * 4 + (size_t)cluster * R * 8 * 4 + (size_t)3 * kFewRows * (R + 8) * 2;
+  return (size_t)kWarps * kFewSlots * 1024 + (size_t)kWarps * kFewRows * kFewPart * 4 + (size_t)cluster * kFewRows * (R + 8) * 4 + (size_t)2 * ((R + 31) / 32) * 1024;
 }
-// The adapter streams through a ring per warp: each lane copies what it will read itself (its 16 bytes of rows g and g + 8), so that nobody waits for
-// anybody, and the second product's first pieces are on their way while the first one's sums are exchanged.
+// The adapter streams through a ring per warp: each lane copies what it will read itself (16 bytes of two of its rows), so that nobody waits for anybody, and
+// the second product's first pieces are on their way while the first one's sums are exchanged.  The adapter's rows are the instruction's columns, tokens its
+// rows: the upper eight rows are empty in the first product, and hold the second piece of u in the second one.
 template <bool kBf16>
 __global__ void __launch_bounds__(kThreads, 2) lora_few_kernel(LoraArgs p) {
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ Tile s_tile;
   __shared__ int s_sum[kWarps];
   __shared__ float s_factor[kFewRows];
-  float* s_part = reinterpret_cast<float*>(smem + kWarps * kFewSlots * 1024);              // [warp][64 ranks][8 rows]
-  float* s_all = s_part + kWarps * kFewRanks * 16 * 8;                                     // [CTA][R][8]
-  uint16_t* s_u = reinterpret_cast<uint16_t*>(s_all + (size_t)p.cluster * p.R * 8);        // [piece][8][R + 8]
+  float* s_part = reinterpret_cast<float*>(smem + kWarps * kFewSlots * 1024);              // [warp][8 rows][kFewPart]
+  float* s_all = s_part + kWarps * kFewRows * kFewPart;                                    // [CTA][8][R + 8]
+  unsigned char* s_u = reinterpret_cast<unsigned char*>(s_all + (size_t)p.cluster * kFewRows * (p.R + 8));  // [two pieces][groups of 32 lanes][16 bytes]
   const int rank_of_cta = blockIdx.x % p.cluster, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   cluster_arrive();  // (waited for before anything is written to another CTA)
   pdl_launch_next();
@@ -227,9 +242,10 @@ __global__ void __launch_bounds__(kThreads, 2) lora_few_kernel(LoraArgs p) {
   unsigned char* ring = smem + warp * kFewSlots * 1024 + lane * 16;
   const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
   int ask_slot = 0, ask_j0 = kb0 < kb1 ? 0 : rank, ask_kb = kb0, ask_i = 0, ask_nt = nt0, ask_j = 0;
-  const size_t eight_a = (size_t)8 * p.K, eight_b = (size_t)8 * p.R;
+  const size_t eight_a = (size_t)8 * p.K, two_b = (size_t)2 * p.R;
+  const int col = 4 * (g >> 1) + (g & 1);  // of sixteen outputs a lane's columns are col and col + 2: it then has four neighbouring ones (see below)
   const uint16_t* ask_a = A + (size_t)g * p.K + kb0 * 32 + 8 * t;  // of rank tile 0 and ask_kb
-  const uint16_t* ask_b = B + (size_t)(nt0 * 16 + g) * p.R;        // of ask_nt
+  const uint16_t* ask_b = B + (size_t)(nt0 * 16 + col) * p.R;      // of ask_nt
   auto ask = [&]() {
     const uint32_t to = ring_at + ask_slot * 1024;
     ask_slot = (ask_slot + 1) % kFewSlots;
@@ -247,10 +263,10 @@ __global__ void __launch_bounds__(kThreads, 2) lora_few_kernel(LoraArgs p) {
         }
       }
     } else if (ask_nt < nt1) {  // of B
-      const uint16_t *from0 = ask_b + ask_j, *from1 = from0 + eight_b;
+      const uint16_t *from0 = ask_b + ask_j, *from1 = from0 + two_b;
       if (ask_nt >= whole) {
-        from0 = B + (size_t)min(ask_nt * 16 + g, p.N - 1) * p.R + ask_j;
-        from1 = B + (size_t)min(ask_nt * 16 + g + 8, p.N - 1) * p.R + ask_j;
+        from0 = B + (size_t)min(ask_nt * 16 + col, p.N - 1) * p.R + ask_j;
+        from1 = B + (size_t)min(ask_nt * 16 + col + 2, p.N - 1) * p.R + ask_j;
       }
       if (ask_j + 32 <= rank)
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n\tcp.async.cg.shared.global [%0+512], [%2], 16;" ::"r"(to), "l"(from0 + 8 * t), "l"(from1 + 8 * t) : "memory");
@@ -260,7 +276,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_few_kernel(LoraArgs p) {
       if (ask_j >= rank) {
         ask_j = 0;
         ++ask_nt;
-        ask_b += 2 * eight_b;
+        ask_b += 8 * two_b;
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -277,56 +293,57 @@ __global__ void __launch_bounds__(kThreads, 2) lora_few_kernel(LoraArgs p) {
   for (int i = 0; i < kFewSlots; ++i) ask();
 
   // ---- u
+  const bool has = g < tile.rows;
   const int8_t* x = p.aq + (size_t)(tile.row + min(g, tile.rows - 1)) * p.K + 8 * t;
-  const float* xs = p.asc + tile.row + min(2 * t, tile.rows - 1);
-  const int second = 2 * t + 1 < tile.rows ? 1 : 0;
+  const float* xs = p.asc + tile.row + min(g, tile.rows - 1);
   for (int j0 = 0; j0 < rank; j0 += kFewRanks * 16) {
-    float acc[kFewRanks][4] = {};
+    float acc[kFewRanks][4] = {};  // row g, ranks 2t, 2t + 1, 8 + 2t, 9 + 2t of the tile
     uint2 v_next = make_uint2(0u, 0u);
-    float s_next[2] = {};
+    float s_next = 0.0f;
     auto values = [&](int kb) {
       if (kb >= kb1) return;
       v_next = *reinterpret_cast<const uint2*>(x + kb * 32);
-      s_next[0] = xs[(size_t)kb * p.Mp];
-      s_next[1] = xs[(size_t)kb * p.Mp + second];
+      s_next = xs[(size_t)kb * p.Mp];
     };
     values(kb0);
     for (int kb = kb0; kb < kb1; kb += kWarps) {
       const uint4 v = eight_of<kBf16>(v_next);
-      const float s0 = s_next[0], s1 = s_next[1];
+      const float s0 = s_next;
       values(kb + kWarps);
 #pragma unroll
       for (int i = 0; i < kFewRanks; ++i)
         if (j0 + i * 16 < rank) {
-          uint4 r0, r1;
-          take(r0, r1);
-          float d[4] = {};
-          mma32<kBf16>(d, r0, r1, v);
-          acc[i][0] = fmaf(s0, d[0], acc[i][0]);
-          acc[i][1] = fmaf(s1, d[1], acc[i][1]);
-          acc[i][2] = fmaf(s0, d[2], acc[i][2]);
-          acc[i][3] = fmaf(s1, d[3], acc[i][3]);
+          uint4 r[2];
+          take(r[0], r[1]);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float d[4] = {};
+            mma32<kBf16>(d, make_uint4(v.x, 0u, v.y, 0u), make_uint4(v.z, 0u, v.w, 0u), r[h]);
+            acc[i][2 * h] = fmaf(s0, d[0], acc[i][2 * h]);
+            acc[i][2 * h + 1] = fmaf(s0, d[1], acc[i][2 * h + 1]);
+          }
         }
     }
 #pragma unroll
     for (int i = 0; i < kFewRanks; ++i)
       if (j0 + i * 16 < rank) {
-        float* to = s_part + (warp * kFewRanks * 16 + i * 16 + g) * 8 + 2 * t;
+        float* to = s_part + (warp * kFewRows + g) * kFewPart + i * 16 + 2 * t;
         *reinterpret_cast<float2*>(to) = make_float2(acc[i][0], acc[i][1]);
-        *reinterpret_cast<float2*>(to + 64) = make_float2(acc[i][2], acc[i][3]);
+        *reinterpret_cast<float2*>(to + 8) = make_float2(acc[i][2], acc[i][3]);
       }
     __syncthreads();
     if (j0 == 0) cluster_wait();  // every CTA has begun
     // the warps' sums, four values per thread, to every CTA
-    const int quads = min(rank - j0, kFewRanks * 16) * 2;
-    if (tid < quads) {
-      float4 v = *reinterpret_cast<const float4*>(s_part + tid * 4);
+    const int row = tid >> 4, j = (tid & 15) * 4;
+    if (row < tile.rows && j0 + j < rank) {
+      const float* from = s_part + row * kFewPart + j;
+      float4 v = *reinterpret_cast<const float4*>(from);
 #pragma unroll
       for (int w = 1; w < kWarps; ++w) {
-        const float4 b = *reinterpret_cast<const float4*>(s_part + w * kFewRanks * 16 * 8 + tid * 4);
+        const float4 b = *reinterpret_cast<const float4*>(from + w * kFewRows * kFewPart);
         v.x += b.x; v.y += b.y; v.z += b.z; v.w += b.w;
       }
-      const float* here = s_all + ((size_t)rank_of_cta * p.R + j0) * 8 + tid * 4;
+      const float* here = s_all + ((size_t)rank_of_cta * kFewRows + row) * (p.R + 8) + j0 + j;
       for (int c = 0; c < p.cluster; ++c) remote_store(at_rank(here, c), v);
     }
     __syncthreads();
@@ -334,61 +351,76 @@ __global__ void __launch_bounds__(kThreads, 2) lora_few_kernel(LoraArgs p) {
   cluster_arrive();
   cluster_wait();
   // ---- the sums of the CTAs in order; a warp per row
-  const int ld = p.R + 8;
-  const size_t piece = (size_t)kFewRows * ld;
-  {
-    const float f = make_pieces<kBf16>(s_u + warp * ld, piece, warp < tile.rows ? rank : 0, rank, [&](int j) {
-      const float* from = s_all + j * 8 + warp;
+  const int chunks = (p.R + 31) / 32;
+  if (warp < tile.rows) {
+    const float f = make_pieces<kBf16>(rank, [&](int j) {
+      const float* from = s_all + warp * (p.R + 8) + j;
       float u = 0.0f;
 #pragma unroll 8
-      for (int c = 0; c < p.cluster; ++c) u += from[(size_t)c * p.R * 8];
+      for (int c = 0; c < p.cluster; ++c) u += from[(size_t)c * kFewRows * (p.R + 8)];
       return u;
+    }, [&](int i, int j, uint16_t v) {
+      const Place at = place_of(j, rank);
+      *reinterpret_cast<uint16_t*>(s_u + ((size_t)(i >> 1) * 2 * chunks + at.group) * 512 + (warp * 4 + at.t) * 16 + (at.value + 2 * (i & 1)) * 2) = v;
     });
     if (lane == 0) s_factor[warp] = f;
   }
   __syncthreads();
 
-  // ---- outputs
-  const float f0 = tile.scale * s_factor[2 * t], f1 = tile.scale * s_factor[2 * t + 1];
-  const bool has0 = 2 * t < tile.rows, has1 = second;
-  const uint16_t* u = s_u + g * ld;
-  const size_t first = (size_t)tile.row + 2 * t;
-  const float* from = p.base ? p.base + first * p.ldb + nt0 * 16 + g : nullptr;
-  float* to = p.C + first * p.ldc + nt0 * 16 + g;
-  float next[4] = {};
+  // ---- outputs: row g, outputs 4t .. 4t + 3 of sixteen
+  const float f = has ? tile.scale * s_factor[g] : 0.0f;
+  const size_t row = (size_t)tile.row + min(g, tile.rows - 1);
+  const bool vec = (((uintptr_t)p.C | (uintptr_t)p.base) & 15) == 0 && ((p.ldc | (p.base ? p.ldb : 0)) & 3) == 0;
+  const float* from = p.base ? p.base + row * p.ldb + nt0 * 16 + 4 * t : nullptr;
+  float* to = p.C + row * p.ldc + nt0 * 16 + 4 * t;
+  float4 next = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   auto load_base = [&](int nt) {
-    if (!from || nt >= nt1) return;
-    const bool n0 = nt < whole || nt * 16 + g < p.N, n1 = nt < whole || nt * 16 + g + 8 < p.N;
-    if (has0 && n0) next[0] = from[0];
-    if (has0 && n1) next[2] = from[8];
-    if (has1 && n0) next[1] = from[p.ldb];
-    if (has1 && n1) next[3] = from[(size_t)p.ldb + 8];
+    if (!from || !has || nt >= nt1) return;
+    if (vec && nt < whole) {
+      next = *reinterpret_cast<const float4*>(from);
+    } else {
+      const int left = p.N - nt * 16 - 4 * t;
+      if (left > 0) next.x = from[0];
+      if (left > 1) next.y = from[1];
+      if (left > 2) next.z = from[2];
+      if (left > 3) next.w = from[3];
+    }
     from += 16;
   };
   load_base(nt0);
+  const unsigned char* u = s_u + lane * 16;
   for (int nt = nt0; nt < nt1; ++nt, to += 16) {
-    const float base[4] = {next[0], next[1], next[2], next[3]};
+    const float4 base = next;
     load_base(nt + 1);
-    float d[4] = {};
+    float d[2][4] = {};
     for (int j = 0; j < rank; j += 32) {
-      uint4 r0, r1;
-      take(r0, r1);
-      if (j + 32 <= rank) {
+      uint4 r[2];
+      take(r[0], r[1]);
 #pragma unroll
-        for (int i = 0; i < kPieces<kBf16>; ++i) mma32<kBf16>(d, r0, r1, *reinterpret_cast<const uint4*>(u + i * piece + j + 8 * t));
-      } else {  // sixteen more
-#pragma unroll
-        for (int i = 0; i < kPieces<kBf16>; ++i) {
-          const uint2 v = *reinterpret_cast<const uint2*>(u + i * piece + j + 4 * t);
-          mma<kBf16>(d, r0.x, r1.x, r0.y, r1.y, v.x, v.y);
+      for (int i = 0; i < (kBf16 ? 2 : 1); ++i) {
+        const unsigned char* of = u + ((size_t)i * 2 * chunks + j / 16) * 512;
+        uint4 lo = *reinterpret_cast<const uint4*>(of), hi = *reinterpret_cast<const uint4*>(of + 512);
+        if (i) lo.y = lo.w = hi.y = hi.w = 0u;  // (the third piece is alone)
+        if (j + 32 <= rank) {
+          mma32<kBf16>(d[0], lo, hi, r[0]);
+          mma32<kBf16>(d[1], lo, hi, r[1]);
+        } else {  // sixteen more
+          mma<kBf16>(d[0], lo.x, lo.y, lo.z, lo.w, r[0].x, r[0].y);
+          mma<kBf16>(d[1], lo.x, lo.y, lo.z, lo.w, r[1].x, r[1].y);
         }
       }
     }
-    const bool n0 = nt < whole || nt * 16 + g < p.N, n1 = nt < whole || nt * 16 + g + 8 < p.N;
-    if (has0 && n0) to[0] = fmaf(f0, d[0], base[0]);
-    if (has0 && n1) to[8] = fmaf(f0, d[2], base[2]);
-    if (has1 && n0) to[p.ldc] = fmaf(f1, d[1], base[1]);
-    if (has1 && n1) to[(size_t)p.ldc + 8] = fmaf(f1, d[3], base[3]);
+    if (!has) continue;
+    const float4 y = make_float4(fmaf(f, d[0][0] + d[0][2], base.x), fmaf(f, d[0][1] + d[0][3], base.y), fmaf(f, d[1][0] + d[1][2], base.z), fmaf(f, d[1][1] + d[1][3], base.w));
+    if (vec && nt < whole) {
+      *reinterpret_cast<float4*>(to) = y;
+    } else {
+      const int left = p.N - nt * 16 - 4 * t;
+      if (left > 0) to[0] = y.x;
+      if (left > 1) to[1] = y.y;
+      if (left > 2) to[2] = y.z;
+      if (left > 3) to[3] = y.w;
+    }
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
@@ -396,11 +428,11 @@ __global__ void __launch_bounds__(kThreads, 2) lora_few_kernel(LoraArgs p) {
 // ---------------------------------------------------------------------------------------------- up to 64 rows
 constexpr int kRows = 64;         // rows of a tile
 constexpr int kCols = 64;         // outputs of a step of the second product
-// u's pieces, A's and B's tiles: rows of whole 64 bytes in 16-byte chunks; where a row is a multiple of 128 bytes odd rows have the halves of their
+// A's and B's tiles: rows of whole 64 bytes in 16-byte chunks; where a row is a multiple of 128 bytes odd rows have the halves of their
 // 128-byte lines changed over, so that two neighbouring rows' 64 bytes lie on different banks.
 struct RowsPlan {
   int groups, parts;                  // warps by ranks (64 each) and by blocks of K in the first product; two more by rows (32 each)
-  int ld, swap;                       // a row of u or B in 16-bit values (a multiple of 32); what odd rows' chunk numbers are xored with
+  int ld, swap;                       // a row of B in 16-bit values (a multiple of 32); what odd rows' chunk numbers are xored with
   int stages2;                        // of asynchronous copies in the second product (three in the first)
   uint32_t stage1, stage2;            // bytes: activations | their scales | A's tile; B's tile | base
   uint32_t all, total1;               // first product: the CTAs' sums lie behind the stages and, over them, the warps' sums
@@ -412,9 +444,9 @@ struct RowsPlan {
     ld = (R + 31) / 32 * 32;
     swap = ld % 64 ? 0 : 4;
     stage1 = parts * (kRows * 32 + kRows * 4 + R * 64);
-    const uint32_t part = (uint32_t)parts * R * kRows * 4;
+    const uint32_t part = (uint32_t)parts * kRows * (R + 8) * 4;
     all = part > 3 * stage1 ? part : 3 * stage1;
-    total1 = all + (uint32_t)R * kRows * 4;
+    total1 = all + (uint32_t)kRows * (R + 8) * 4;
     pieces = (bf16 ? 3 : 2) * kRows * ld * 2;
     stage2 = kCols * ld * 2 + kRows * kCols * 4;
     stages2 = R <= 128 ? 3 : 2;
@@ -442,8 +474,9 @@ __global__ void __launch_bounds__(kThreads, 2) lora_inner_kernel(LoraArgs p, Row
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ Tile s_tile;
   __shared__ int s_sum[kWarps];
-  float* s_part = reinterpret_cast<float*>(smem);              // [K part][R][64 rows]
-  float* s_all = reinterpret_cast<float*>(smem + plan.all);    // [CTA][R][rows that the CTA joins]
+  float* s_part = reinterpret_cast<float*>(smem);              // [K part][64 rows][R + 8]
+  float* s_all = reinterpret_cast<float*>(smem + plan.all);    // [CTA][rows that this CTA joins][R + 8]
+  const int ldp = p.R + 8;
   const int index = blockIdx.x / p.cluster, rank_of_cta = blockIdx.x % p.cluster, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   cluster_arrive();
   pdl_wait();
@@ -486,7 +519,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_inner_kernel(LoraArgs p, Row
       }
       copies_begun();
     };
-    float acc[4][4][4] = {};
+    float acc[2][8][4] = {};  // rows 16 m + g, + 8, ranks 8 i + 2t, 2t + 1
     ask(0, 0);
     ask(1, 1);
     for (int step = 0, stage = 0; step < steps; ++step) {
@@ -497,74 +530,80 @@ __global__ void __launch_bounds__(kThreads, 2) lora_inner_kernel(LoraArgs p, Row
       stage = stage == 2 ? 0 : stage + 1;
       if (j0 >= rank || kb0 + step * parts + part >= kb1 || r0 >= tile.rows) continue;
       const uint2* x = reinterpret_cast<const uint2*>(here + part * kRows * 32) + (r0 + g) * 4 + t;
-      const float2* xs = reinterpret_cast<const float2*>(here + scales_at + part * kRows * 4 + r0 * 4) + t;
+      const float* xs = reinterpret_cast<const float*>(here + scales_at + part * kRows * 4) + r0 + g;
       const uint4* a = reinterpret_cast<const uint4*>(here + a_at) + ((size_t)(j0 + g) << row_log) + ((part * 4) ^ (g & 1 ? swap : 0)) + t;
-      uint4 c[4];
-      float2 sc[4];
+      uint4 lo[2], hi[2];
+      float sc[2][2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        c[i] = eight_of<kBf16>(x[i * 32]);
-        sc[i] = xs[i * 4];
+      for (int m = 0; m < 2; ++m) {
+        const uint4 v = eight_of<kBf16>(x[m * 64]), w = eight_of<kBf16>(x[m * 64 + 32]);
+        lo[m] = make_uint4(v.x, w.x, v.y, w.y);
+        hi[m] = make_uint4(v.z, w.z, v.w, w.w);
+        sc[m][0] = xs[16 * m];
+        sc[m][1] = xs[16 * m + 8];
       }
 #pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        if (j0 + 16 * m >= rank) break;
-        const uint4 a0 = a[(16 * m) << row_log], a1 = a[(16 * m + 8) << row_log];
+      for (int i = 0; i < 8; ++i) {
+        if (j0 + 8 * i >= rank) break;
+        const uint4 c = a[(8 * i) << row_log];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int m = 0; m < 2; ++m) {
           float d[4] = {};
-          mma32<kBf16>(d, a0, a1, c[i]);
-          acc[m][i][0] = fmaf(sc[i].x, d[0], acc[m][i][0]);
-          acc[m][i][1] = fmaf(sc[i].y, d[1], acc[m][i][1]);
-          acc[m][i][2] = fmaf(sc[i].x, d[2], acc[m][i][2]);
-          acc[m][i][3] = fmaf(sc[i].y, d[3], acc[m][i][3]);
+          mma32<kBf16>(d, lo[m], hi[m], c);
+          acc[m][i][0] = fmaf(sc[m][0], d[0], acc[m][i][0]);
+          acc[m][i][1] = fmaf(sc[m][0], d[1], acc[m][i][1]);
+          acc[m][i][2] = fmaf(sc[m][1], d[2], acc[m][i][2]);
+          acc[m][i][3] = fmaf(sc[m][1], d[3], acc[m][i][3]);
         }
       }
     }
     copies_there<0>();
     __syncthreads();  // (the partial sums go over the stages)
 #pragma unroll
-    for (int m = 0; m < 4; ++m)
-      if (j0 + 16 * m < rank)
+    for (int i = 0; i < 8; ++i)
+      if (j0 + 8 * i < rank)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float* to = s_part + ((size_t)part * p.R + j0 + 16 * m + g) * kRows + r0 + 8 * i + 2 * t;
+        for (int m = 0; m < 2; ++m) {
+          float* to = s_part + (size_t)(part * kRows + r0 + 16 * m + g) * ldp + j0 + 8 * i + 2 * t;
           *reinterpret_cast<float2*>(to) = make_float2(acc[m][i][0], acc[m][i][1]);
-          *reinterpret_cast<float2*>(to + 8 * kRows) = make_float2(acc[m][i][2], acc[m][i][3]);
+          *reinterpret_cast<float2*>(to + 8 * ldp) = make_float2(acc[m][i][2], acc[m][i][3]);
         }
   }
   __syncthreads();
   cluster_wait();  // every CTA has begun
-  // the CTA's sums, four rows per thread, to the CTA that joins these rows
+  // the CTA's sums, four ranks per thread, to the CTA that joins these rows
   const int own = kRows / p.cluster;  // (8, 16, 32 or 64)
-  for (int i = tid; i < rank * (kRows / 4); i += kThreads) {
-    const int j = i / (kRows / 4), row = i % (kRows / 4) * 4;
-    float4 v = *reinterpret_cast<const float4*>(s_part + (size_t)j * kRows + row);
-    for (int w = 1; w < parts; ++w) {
-      const float4 b = *reinterpret_cast<const float4*>(s_part + ((size_t)w * p.R + j) * kRows + row);
-      v.x += b.x; v.y += b.y; v.z += b.z; v.w += b.w;
+  {
+    const int row = tid >> 2;
+    for (int j = (tid & 3) * 4; j < rank && row < tile.rows; j += 16) {
+      const float* from = s_part + (size_t)row * ldp + j;
+      float4 v = *reinterpret_cast<const float4*>(from);
+      for (int w = 1; w < parts; ++w) {
+        const float4 b = *reinterpret_cast<const float4*>(from + (size_t)w * kRows * ldp);
+        v.x += b.x; v.y += b.y; v.z += b.z; v.w += b.w;
+      }
+      remote_store(at_rank(s_all + ((size_t)rank_of_cta * own + (row & (own - 1))) * ldp + j, row / own), v);
     }
-    remote_store(at_rank(s_all + ((size_t)rank_of_cta * p.R + j) * own + (row & (own - 1)), row / own), v);
   }
   cluster_arrive();
   cluster_wait();
-  // ---- a warp per row of its CTA: the sums of the CTAs in order
-  uint16_t* u = reinterpret_cast<uint16_t*>(scratch + plan.at_pieces + (size_t)index * plan.pieces);
+  // ---- a warp per row of its CTA: the sums of the CTAs in order.  The pieces lie as the second product's instructions take them: [piece][16 rows][32 lanes' 16
+  // bytes per instruction]
+  unsigned char* u = scratch + plan.at_pieces + (size_t)index * plan.pieces;
   float* factors = reinterpret_cast<float*>(scratch + plan.at_factors) + (size_t)index * kRows;
   for (int i = warp; i < own; i += kWarps) {
     const int row = rank_of_cta * own + i;
-    if (row >= tile.rows) {
-      for (int k = lane; k < kPieces<kBf16> * plan.ld; k += 32) u[(size_t)(k / plan.ld) * kRows * plan.ld + row * plan.ld + k % plan.ld] = 0;
-      if (lane == 0) factors[row] = 0.0f;
-      continue;
-    }
-    const float f = make_pieces<kBf16>(u + row * plan.ld, (size_t)kRows * plan.ld, rank, plan.ld, [&](int j) {
-      const float* from = s_all + (size_t)j * own + i;
+    if (row >= tile.rows) break;
+    const float f = make_pieces<kBf16>(rank, [&](int j) {
+      const float* from = s_all + (size_t)i * ldp + j;
       float sum = 0.0f;
 #pragma unroll 8
-      for (int c = 0; c < p.cluster; ++c) sum += from[(size_t)c * p.R * own];
+      for (int c = 0; c < p.cluster; ++c) sum += from[(size_t)c * own * ldp];
       return sum;
-    }, (row & 1 ? plan.swap : 0) * 8);
+    }, [&](int k, int j, uint16_t v) {
+      const Place at = place_of(j, rank);
+      *reinterpret_cast<uint16_t*>(u + ((size_t)(k * 4 + (row >> 4)) * (plan.ld / 16) + at.group) * 512 + ((row & 7) * 4 + at.t) * 16 + (at.value + (row & 8 ? 2 : 0)) * 2) = v;
+    });
     if (lane == 0) factors[row] = tile.scale * f;
   }
 }
@@ -576,7 +615,6 @@ __global__ void __launch_bounds__(kThreads, 2) lora_outer_kernel(LoraArgs p, Row
   extern __shared__ __align__(16) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3, ld = plan.ld;
   const int m0 = (warp & 3) * 16, half = (warp >> 2) * 32;  // a warp has 16 rows and 32 of the 64 outputs
-  const uint16_t* s_u = reinterpret_cast<const uint16_t*>(smem);
   const uint32_t smem_at = (uint32_t)__cvta_generic_to_shared(smem), stages_at = smem_at + plan.pieces;
   const bool in_place = p.base == p.C;
   pdl_launch_next();
@@ -587,10 +625,9 @@ __global__ void __launch_bounds__(kThreads, 2) lora_outer_kernel(LoraArgs p, Row
   if (begin >= end) return;
   const Tile* tiles = reinterpret_cast<const Tile*>(scratch + plan.at_tiles);
 
-  const size_t piece = (size_t)kRows * ld;
   const int col = 4 * (g >> 1) + (g & 1);     // column g of the first instruction; of the second one: two further
-  const int swap = g & 1 ? plan.swap : 0;     // (rows g + 8, columns two further: as odd as g)
-  const uint16_t *u0 = s_u + (m0 + g) * ld + t * 8, *u1 = u0 + 8 * ld;
+  const int swap = g & 1 ? plan.swap : 0;     // (columns two further are as odd as g)
+  auto of_u = [&](int k, int group) { return *reinterpret_cast<const uint4*>(smem + ((k * 4 + (warp & 3)) * (ld / 16) + group) * 512 + lane * 16); };
   const int b_row = tid >> 2, b_chunk = tid & 3;  // four threads copy a row of B
   const uint32_t b_to = stages_at + (b_row * ld + (b_chunk ^ (b_row & 1 ? plan.swap : 0)) * 8) * 2, b_swap = b_row & 1 && plan.swap ? 0xFFFFFFC0u : 64u;  // (the next four chunks)
   const uint32_t base_to = stages_at + kCols * ld * 2 + tid * 16;
@@ -679,8 +716,8 @@ __global__ void __launch_bounds__(kThreads, 2) lora_outer_kernel(LoraArgs p, Row
           if (32 * j < ld)
 #pragma unroll
             for (int k = 0; k < kPieces<kBf16>; ++k) {
-              held[kRegs ? j : 0][k][0] = *reinterpret_cast<const uint4*>(u0 + k * piece + (4 * j ^ swap) * 8);
-              held[kRegs ? j : 0][k][1] = *reinterpret_cast<const uint4*>(u1 + k * piece + (4 * j ^ swap) * 8);
+              held[kRegs ? j : 0][k][0] = of_u(k, 2 * j);
+              held[kRegs ? j : 0][k][1] = of_u(k, 2 * j + 1);
             }
       }
     }
@@ -726,7 +763,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_outer_kernel(LoraArgs p, Row
             for (int q = 0; q < 2; ++q) v[h][q] = *reinterpret_cast<const uint4*>(of_b(h, q, j / 8));
 #pragma unroll
           for (int k = 0; k < kPieces<kBf16>; ++k) {
-            const uint4 r0 = *reinterpret_cast<const uint4*>(u0 + k * piece + (j / 8 ^ swap) * 8), r1 = *reinterpret_cast<const uint4*>(u1 + k * piece + (j / 8 ^ swap) * 8);
+            const uint4 r0 = of_u(k, j / 16), r1 = of_u(k, j / 16 + 1);
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -737,13 +774,13 @@ __global__ void __launch_bounds__(kThreads, 2) lora_outer_kernel(LoraArgs p, Row
         const int at = (j / 8 ^ swap) * 8 + 4 * t - 8 * t;
 #pragma unroll
         for (int k = 0; k < kPieces<kBf16>; ++k) {
-          const uint2 r0 = *reinterpret_cast<const uint2*>(u0 + k * piece + at), r1 = *reinterpret_cast<const uint2*>(u1 + k * piece + at);
+          const uint4 r = of_u(k, j / 16);
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
               const uint2 v = *reinterpret_cast<const uint2*>(b + (16 * h + 2 * q) * ld + at);
-              mma<kBf16>(d[h][q], r0.x, r1.x, r0.y, r1.y, v.x, v.y);
+              mma<kBf16>(d[h][q], r.x, r.y, r.z, r.w, v.x, v.y);
             }
         }
       }
@@ -817,7 +854,7 @@ extern "C" int izb_lora_add(int dtype, const void* d_A, const void* d_B, int n_a
     for (auto kernel : {lora_few_kernel<false>, lora_few_kernel<true>}) {
       static izb_device_once once[2];
       if (int rc = once[kernel == lora_few_kernel<true>].run(device, [&]() -> int {
-            IZB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)few_smem(kMaxRank, kMaxCluster)));
+            IZB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(few_smem(kMaxRank, 8) > few_smem(128, 16) ? few_smem(kMaxRank, 8) : few_smem(128, 16))));
             IZB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
             return IZB_OK;
           }))
