@@ -88,6 +88,19 @@ __device__ __forceinline__ Tile find_tile(const LoraArgs& p, int tile, Tile* s_t
 
 // ---------------------------------------------------------------------------------------------- operands
 template <bool kBf16>
+__device__ __forceinline__ float2 two_values(uint32_t w) {
+  if (kBf16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {  // two IEEE operations in one instruction
+  unsigned long long r;
+  asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %4};\n\tmov.b64 c, {%5, %6};\n\tfma.rn.f32x2 %0, a, b, c;\n\t}"
+      : "=l"(r) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  float2 o;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(o.x), "=f"(o.y) : "l"(r));
+  return o;
+}
+template <bool kBf16>
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   if (kBf16)
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -176,6 +189,18 @@ __device__ __forceinline__ float make_pieces(int rank, Sum sum, Put put) {
   return ldexpf(1.0f, ex - 13);
 }
 
+// ---------------------------------------------------------------------------------------------- asynchronous copies
+template <int kN>
+__device__ __forceinline__ void copies_there() { asm volatile("cp.async.wait_group %0;" ::"n"(kN) : "memory"); }
+__device__ __forceinline__ void copies_there(int later) {
+  if (later == 2) copies_there<2>();
+  else if (later == 1) copies_there<1>();
+  else copies_there<0>();
+}
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
+__device__ __forceinline__ void copy4(uint32_t to, const void* from) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory"); }
+__device__ __forceinline__ void copies_begun() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+
 // ---------------------------------------------------------------------------------------------- clusters
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
@@ -202,11 +227,12 @@ __device__ __forceinline__ void copy_base(const LoraArgs& p, const Tile& tile, i
 // ---------------------------------------------------------------------------------------------- up to 8 rows
 constexpr int kFewRows = 8;
 constexpr int kFewRanks = 4;   // rank tiles of 16 at a time
-constexpr int kFewSlots = 8;   // pieces of an adapter (16 rows x 32 elements, 1 KB) that a warp has asked for: 64 KB per CTA
+constexpr int kFewSlots = 6;   // pieces of an adapter (16 rows x 32 elements, 1 KB, and 16 bytes of the base per lane) that a warp has asked for: 72 KB per CTA
+constexpr int kFewSlot = 1536;
 constexpr int kFewPart = kFewRanks * 16 + 8;  // a row of partial sums (the padding: rows on different banks)
 // rings | partial sums of the warps | those of the CTAs | the pieces of u, two to an instruction
 static size_t few_smem(int R, int cluster) {
-  return (size_t)kWarps * kFewSlots * 1024 + (size_t)kWarps * kFewRows * kFewPart * 4 + (size_t)cluster * kFewRows * (R + 8) * 4 + (size_t)2 * ((R + 31) / 32) * 1024;
+  return (size_t)kWarps * kFewSlots * kFewSlot + (size_t)kWarps * kFewRows * kFewPart * 4 + (size_t)cluster * kFewRows * (R + 8) * 4 + (size_t)2 * ((R + 31) / 32) * 1024;
 }
 // The adapter streams through a ring per warp: each lane copies what it will read itself (16 bytes of two of its rows), so that nobody waits for anybody, and
 // the second product's first pieces are on their way while the first one's sums are exchanged.  The adapter's rows are the instruction's columns, tokens its
@@ -217,7 +243,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_few_kernel(LoraArgs p) {
   __shared__ Tile s_tile;
   __shared__ int s_sum[kWarps];
   __shared__ float s_factor[kFewRows];
-  float* s_part = reinterpret_cast<float*>(smem + kWarps * kFewSlots * 1024);              // [warp][8 rows][kFewPart]
+  float* s_part = reinterpret_cast<float*>(smem + kWarps * kFewSlots * kFewSlot);              // [warp][8 rows][kFewPart]
   float* s_all = s_part + kWarps * kFewRows * kFewPart;                                    // [CTA][8][R + 8]
   unsigned char* s_u = reinterpret_cast<unsigned char*>(s_all + (size_t)p.cluster * kFewRows * (p.R + 8));  // [two pieces][groups of 32 lanes][16 bytes]
   const int rank_of_cta = blockIdx.x % p.cluster, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -235,20 +261,34 @@ __global__ void __launch_bounds__(kThreads, 2) lora_few_kernel(LoraArgs p) {
   const int rank = (tile.rank + 15) & ~15;  // (the rows in between are zeros)
   // this warp's 32-blocks of K and its sixteens of outputs
   const int kb1 = share(p.K / 32, p.cluster, rank_of_cta + 1), kb0 = share(p.K / 32, p.cluster, rank_of_cta) + warp;
-  const int tiles = (p.N + 15) / 16, nt0 = share(tiles, p.cluster * kWarps, rank_of_cta * kWarps + warp), nt1 = share(tiles, p.cluster * kWarps, rank_of_cta * kWarps + warp + 1);
-  const int whole = p.N / 16;  // (a last tile may be cut off)
+  // (A single row is dealt with in f32 -- an instruction for eight rows would be an eighth of its own worth: two lanes on an output up to rank 16, else four, of
+  // which each has 8 elements of a piece's 16, 32 or, beyond that, two times 8 of 64.)
+  const bool single = tile.rows == 1, split = single && rank > 32;
+  const int lanes_log = rank <= 16 ? 1 : 2, lanes = 1 << lanes_log, unit = !single ? 16 : split ? 8 : 64 >> lanes_log;
+  const int tiles = (p.N + unit - 1) / unit, nt0 = share(tiles, p.cluster * kWarps, rank_of_cta * kWarps + warp), nt1 = share(tiles, p.cluster * kWarps, rank_of_cta * kWarps + warp + 1);
+  const int whole = p.N / unit;  // (a last tile may be cut off)
 
   // ---- the ring: pieces in the order in which they are used below
-  unsigned char* ring = smem + warp * kFewSlots * 1024 + lane * 16;
+  unsigned char* ring = smem + warp * kFewSlots * kFewSlot + lane * 16;
   const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
   int ask_slot = 0, ask_j0 = kb0 < kb1 ? 0 : rank, ask_kb = kb0, ask_i = 0, ask_nt = nt0, ask_j = 0;
-  const size_t eight_a = (size_t)8 * p.K, two_b = (size_t)2 * p.R;
-  const int col = 4 * (g >> 1) + (g & 1);  // of sixteen outputs a lane's columns are col and col + 2: it then has four neighbouring ones (see below)
+  const size_t eight_a = (size_t)8 * p.K;
+  // of sixteen outputs a lane's columns are col and col + 2: it then has four neighbouring ones (see below)
+  const int col = single ? lane >> lanes_log : 4 * (g >> 1) + (g & 1), col_step = !single ? 2 : split ? 0 : unit / 2;
+  const size_t step_b = (size_t)col_step * p.R, unit_b = (size_t)unit * p.R;
   const uint16_t* ask_a = A + (size_t)g * p.K + kb0 * 32 + 8 * t;  // of rank tile 0 and ask_kb
-  const uint16_t* ask_b = B + (size_t)(nt0 * 16 + col) * p.R;      // of ask_nt
+  const uint16_t* ask_b = B + (size_t)(nt0 * unit + col) * p.R;    // of ask_nt
+  // A lane's outputs: row g, four neighbouring ones of sixteen.  Of a single row: where the halves of a piece are two outputs, the sum over the lanes that share
+  // them leaves the second one with those of the upper half.
+  const bool upper = !split && lane & (lanes >> 1), mine_has = single ? (split ? (lane & 3) == 0 : (lane & ((lanes >> 1) - 1)) == 0) : g < tile.rows;
+  const int out_at = single ? (upper ? col_step : 0) + col : 4 * t;
+  const size_t out_row = (size_t)tile.row + (single ? 0 : min(g, tile.rows - 1));
+  const bool vec = (((uintptr_t)p.C | (uintptr_t)p.base) & 15) == 0 && ((p.ldc | (p.base ? p.ldb : 0)) & 3) == 0;
+  const float* ask_base = p.base + out_row * p.ldb + nt0 * unit + out_at;  // (not looked at without a base)
+  float* to = p.C + out_row * p.ldc + nt0 * unit + out_at;
   auto ask = [&]() {
-    const uint32_t to = ring_at + ask_slot * 1024;
-    ask_slot = (ask_slot + 1) % kFewSlots;
+    const uint32_t to = ring_at + ask_slot * kFewSlot;
+    ask_slot = ask_slot + 1 == kFewSlots ? 0 : ask_slot + 1;
     if (ask_j0 < rank) {  // of A
       const uint16_t* from = ask_a + 2 * (ask_j0 / 16 + ask_i) * eight_a;
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n\tcp.async.cg.shared.global [%0+512], [%2], 16;" ::"r"(to), "l"(from), "l"(from + eight_a) : "memory");
@@ -263,37 +303,59 @@ __global__ void __launch_bounds__(kThreads, 2) lora_few_kernel(LoraArgs p) {
         }
       }
     } else if (ask_nt < nt1) {  // of B
-      const uint16_t *from0 = ask_b + ask_j, *from1 = from0 + two_b;
+      const uint16_t *from0 = ask_b + ask_j, *from1 = from0 + step_b;
       if (ask_nt >= whole) {
-        from0 = B + (size_t)min(ask_nt * 16 + col, p.N - 1) * p.R + ask_j;
-        from1 = B + (size_t)min(ask_nt * 16 + col + 2, p.N - 1) * p.R + ask_j;
+        from0 = B + (size_t)min(ask_nt * unit + col, p.N - 1) * p.R + ask_j;
+        from1 = B + (size_t)min(ask_nt * unit + col + col_step, p.N - 1) * p.R + ask_j;
       }
-      if (ask_j + 32 <= rank)
+      if (ask_j == 0 && p.base && mine_has) {  // what this lane will add
+        const bool cut = ask_nt >= whole;
+        const int n = ask_nt * unit + out_at;
+        if (single) {
+          if (!cut || n < p.N) copy4(to + 1024, ask_base);
+        } else if (vec && !cut) {
+          copy16(to + 1024, ask_base);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (n + k < p.N) copy4(to + 1024 + 4 * k, ask_base + k);
+        }
+      }
+      if (single) {  // (past the rank: zeros)
+        const int j0 = (lane & (lanes - 1)) * 8, j1 = split ? j0 + 32 : j0, bytes0 = ask_j + j0 < rank ? 16 : 0, bytes1 = ask_j + j1 < rank ? 16 : 0;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %3;\n\tcp.async.cg.shared.global [%0+512], [%2], 16, %4;" ::"r"(to), "l"(from0 + (bytes0 ? j0 : 0)),
+                     "l"(from1 + (bytes1 ? j1 : 0)), "r"(bytes0), "r"(bytes1)
+                     : "memory");
+        ask_j += 64;
+      } else if (ask_j + 32 <= rank) {
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n\tcp.async.cg.shared.global [%0+512], [%2], 16;" ::"r"(to), "l"(from0 + 8 * t), "l"(from1 + 8 * t) : "memory");
-      else
+        ask_j += 32;
+      } else {
         asm volatile("cp.async.ca.shared.global [%0], [%1], 8;\n\tcp.async.ca.shared.global [%0+512], [%2], 8;" ::"r"(to), "l"(from0 + 4 * t), "l"(from1 + 4 * t) : "memory");
-      ask_j += 32;
+        ask_j += 32;
+      }
       if (ask_j >= rank) {
         ask_j = 0;
         ++ask_nt;
-        ask_b += 8 * two_b;
+        ask_b += unit_b;
+        ask_base += unit;
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
   int slot = 0;
-  auto take = [&](uint4& r0, uint4& r1) {
+  auto take = [&](uint4& r0, uint4& r1, float4& base) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kFewSlots - 1) : "memory");
-    r0 = *reinterpret_cast<const uint4*>(ring + slot * 1024);
-    r1 = *reinterpret_cast<const uint4*>(ring + slot * 1024 + 512);
-    slot = (slot + 1) % kFewSlots;
+    r0 = *reinterpret_cast<const uint4*>(ring + slot * kFewSlot);
+    r1 = *reinterpret_cast<const uint4*>(ring + slot * kFewSlot + 512);
+    base = *reinterpret_cast<const float4*>(ring + slot * kFewSlot + 1024);  // (of an output's first piece)
+    slot = slot + 1 == kFewSlots ? 0 : slot + 1;
     ask();
   };
 #pragma unroll
   for (int i = 0; i < kFewSlots; ++i) ask();
 
   // ---- u
-  const bool has = g < tile.rows;
   const int8_t* x = p.aq + (size_t)(tile.row + min(g, tile.rows - 1)) * p.K + 8 * t;
   const float* xs = p.asc + tile.row + min(g, tile.rows - 1);
   for (int j0 = 0; j0 < rank; j0 += kFewRanks * 16) {
@@ -314,7 +376,8 @@ __global__ void __launch_bounds__(kThreads, 2) lora_few_kernel(LoraArgs p) {
       for (int i = 0; i < kFewRanks; ++i)
         if (j0 + i * 16 < rank) {
           uint4 r[2];
-          take(r[0], r[1]);
+          float4 none;
+          take(r[0], r[1], none);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             float d[4] = {};
@@ -350,6 +413,60 @@ __global__ void __launch_bounds__(kThreads, 2) lora_few_kernel(LoraArgs p) {
   }
   cluster_arrive();
   cluster_wait();
+  // ---- a single row: its sums as they are, and outputs by lanes that share a row of B
+  if (single) {
+    float* s_f = reinterpret_cast<float*>(s_u);
+    for (int j = tid; j < ((rank + 63) & ~63); j += kThreads) {
+      float u = 0.0f;
+      if (j < rank)
+#pragma unroll 8
+        for (int c = 0; c < p.cluster; ++c) u += s_all[(size_t)c * kFewRows * (p.R + 8) + j];
+      s_f[j] = u;
+    }
+    __syncthreads();
+    const float* mine = s_f + (lane & (lanes - 1)) * 8;
+    float2 u[2][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) u[h][e] = *reinterpret_cast<const float2*>(mine + (split ? 32 * h : 0) + 2 * e);
+#pragma unroll 2
+    for (int nt = nt0; nt < nt1; ++nt, to += unit) {
+      float base = 0.0f;
+      float2 v[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+      for (int j = 0; j < rank; j += 64) {
+        uint4 r[2];
+        float4 here;
+        take(r[0], r[1], here);
+        if (j == 0 && p.base) base = here.x;
+        if (rank > 64) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) u[h][e] = *reinterpret_cast<const float2*>(mine + j + 32 * h + 2 * e);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t w[4] = {r[h].x, r[h].y, r[h].z, r[h].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[h] = fma2(two_values<kBf16>(w[e]), u[h][e], v[h]);
+        }
+      }
+      const float a = v[0].x + v[0].y, b = v[1].x + v[1].y;
+      float y;
+      if (split) {
+        y = a + b;
+        y += __shfl_xor_sync(0xFFFFFFFFu, y, 2);
+        y += __shfl_xor_sync(0xFFFFFFFFu, y, 1);
+      } else {
+        y = (upper ? b : a) + __shfl_xor_sync(0xFFFFFFFFu, upper ? a : b, lanes >> 1);
+        if (lanes == 4) y += __shfl_xor_sync(0xFFFFFFFFu, y, 1);
+      }
+      if (mine_has && (nt < whole || nt * unit + out_at < p.N)) *to = fmaf(tile.scale, y, base);
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    return;
+  }
   // ---- the sums of the CTAs in order; a warp per row
   const int chunks = (p.R + 31) / 32;
   if (warp < tile.rows) {
@@ -367,35 +484,17 @@ __global__ void __launch_bounds__(kThreads, 2) lora_few_kernel(LoraArgs p) {
   }
   __syncthreads();
 
-  // ---- outputs: row g, outputs 4t .. 4t + 3 of sixteen
-  const float f = has ? tile.scale * s_factor[g] : 0.0f;
-  const size_t row = (size_t)tile.row + min(g, tile.rows - 1);
-  const bool vec = (((uintptr_t)p.C | (uintptr_t)p.base) & 15) == 0 && ((p.ldc | (p.base ? p.ldb : 0)) & 3) == 0;
-  const float* from = p.base ? p.base + row * p.ldb + nt0 * 16 + 4 * t : nullptr;
-  float* to = p.C + row * p.ldc + nt0 * 16 + 4 * t;
-  float4 next = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  auto load_base = [&](int nt) {
-    if (!from || !has || nt >= nt1) return;
-    if (vec && nt < whole) {
-      next = *reinterpret_cast<const float4*>(from);
-    } else {
-      const int left = p.N - nt * 16 - 4 * t;
-      if (left > 0) next.x = from[0];
-      if (left > 1) next.y = from[1];
-      if (left > 2) next.z = from[2];
-      if (left > 3) next.w = from[3];
-    }
-    from += 16;
-  };
-  load_base(nt0);
+  // ---- outputs
+  const float f = mine_has ? tile.scale * s_factor[g] : 0.0f;
   const unsigned char* u = s_u + lane * 16;
   for (int nt = nt0; nt < nt1; ++nt, to += 16) {
-    const float4 base = next;
-    load_base(nt + 1);
+    float4 base = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     float d[2][4] = {};
     for (int j = 0; j < rank; j += 32) {
       uint4 r[2];
-      take(r[0], r[1]);
+      float4 here;
+      take(r[0], r[1], here);
+      if (j == 0 && p.base) base = here;
 #pragma unroll
       for (int i = 0; i < (kBf16 ? 2 : 1); ++i) {
         const unsigned char* of = u + ((size_t)i * 2 * chunks + j / 16) * 512;
@@ -410,7 +509,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_few_kernel(LoraArgs p) {
         }
       }
     }
-    if (!has) continue;
+    if (!mine_has) continue;
     const float4 y = make_float4(fmaf(f, d[0][0] + d[0][2], base.x), fmaf(f, d[0][1] + d[0][3], base.y), fmaf(f, d[1][0] + d[1][2], base.z), fmaf(f, d[1][1] + d[1][3], base.w));
     if (vec && nt < whole) {
       *reinterpret_cast<float4*>(to) = y;
@@ -457,17 +556,6 @@ struct RowsPlan {
   }
   size_t scratch(size_t tiles) const { return at_pieces + tiles * pieces; }
 };
-template <int kN>
-__device__ __forceinline__ void copies_there() { asm volatile("cp.async.wait_group %0;" ::"n"(kN) : "memory"); }
-__device__ __forceinline__ void copies_there(int later) {
-  if (later == 2) copies_there<2>();
-  else if (later == 1) copies_there<1>();
-  else copies_there<0>();
-}
-__device__ __forceinline__ void copy16(uint32_t to, const void* from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
-__device__ __forceinline__ void copy4(uint32_t to, const void* from) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory"); }
-__device__ __forceinline__ void copies_begun() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-
 // The first product: u's pieces, rows' factors and the tile's place, into scratch.
 template <bool kBf16>
 __global__ void __launch_bounds__(kThreads, 2) lora_inner_kernel(LoraArgs p, RowsPlan plan, unsigned char* scratch) {
