@@ -227,30 +227,37 @@ __device__ __forceinline__ void copy_base(const LoraArgs& p, const Tile& tile, i
 // ---------------------------------------------------------------------------------------------- up to 8 rows
 constexpr int kFewRows = 8;
 constexpr int kFewRanks = 4;   // rank tiles of 16 at a time
-constexpr int kFewSlots = 6;   // pieces of an adapter (16 rows x 32 elements, 1 KB, and 16 bytes of the base per lane) that a warp has asked for: 72 KB per CTA
-constexpr int kFewSlot = 1536;
+// Pieces of an adapter (16 rows x 32 elements, 1 KB, and what the base has for them: 16 bytes per lane, of a single row 4) that a warp has asked for
+template <int kRowsOf>
+constexpr int kFewSlots = kRowsOf == 1 ? 5 : 6;
+template <int kRowsOf>
+constexpr int kFewSlot = kRowsOf == 1 ? 1152 : 1536;
+template <int kRowsOf>
+constexpr int kFewBlocks = kRowsOf == 1 ? 3 : 2;  // CTAs per multiprocessor
 constexpr int kFewPart = kFewRanks * 16 + 8;  // a row of partial sums (the padding: rows on different banks)
 // rings | partial sums of the warps | those of the CTAs | the pieces of u, two to an instruction
+template <int kRowsOf>
 static size_t few_smem(int R, int cluster) {
-  return (size_t)kWarps * kFewSlots * kFewSlot + (size_t)kWarps * kFewRows * kFewPart * 4 + (size_t)cluster * kFewRows * (R + 8) * 4 + (size_t)2 * ((R + 31) / 32) * 1024;
+  return (size_t)kWarps * kFewSlots<kRowsOf> * kFewSlot<kRowsOf> + (size_t)kWarps * kRowsOf * kFewPart * 4 + (size_t)cluster * kRowsOf * (R + 8) * 4 + (size_t)2 * ((R + 31) / 32) * 1024;
 }
 // The adapter streams through a ring per warp: each lane copies what it will read itself (16 bytes of two of its rows), so that nobody waits for anybody, and
 // the second product's first pieces are on their way while the first one's sums are exchanged.  The adapter's rows are the instruction's columns, tokens its
 // rows: the upper eight rows are empty in the first product, and hold the second piece of u in the second one.
-template <bool kBf16>
-__global__ void __launch_bounds__(kThreads, 2) lora_few_kernel(LoraArgs p) {
+template <bool kBf16, int kRowsOf>
+__global__ void __launch_bounds__(kThreads, kFewBlocks<kRowsOf>) lora_few_kernel(LoraArgs p) {
+  constexpr int kSlots = kFewSlots<kRowsOf>, kSlot = kFewSlot<kRowsOf>;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ Tile s_tile;
   __shared__ int s_sum[kWarps];
-  __shared__ float s_factor[kFewRows];
-  float* s_part = reinterpret_cast<float*>(smem + kWarps * kFewSlots * kFewSlot);              // [warp][8 rows][kFewPart]
-  float* s_all = s_part + kWarps * kFewRows * kFewPart;                                    // [CTA][8][R + 8]
-  unsigned char* s_u = reinterpret_cast<unsigned char*>(s_all + (size_t)p.cluster * kFewRows * (p.R + 8));  // [two pieces][groups of 32 lanes][16 bytes]
+  __shared__ float s_factor[kRowsOf];
+  float* s_part = reinterpret_cast<float*>(smem + kWarps * kSlots * kSlot);              // [warp][rows][kFewPart]
+  float* s_all = s_part + kWarps * kRowsOf * kFewPart;                                    // [CTA][rows][R + 8]
+  unsigned char* s_u = reinterpret_cast<unsigned char*>(s_all + (size_t)p.cluster * kRowsOf * (p.R + 8));  // [two pieces][groups of 32 lanes][16 bytes]
   const int rank_of_cta = blockIdx.x % p.cluster, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   cluster_arrive();  // (waited for before anything is written to another CTA)
   pdl_launch_next();
   pdl_wait();
-  const Tile tile = find_tile<kFewRows>(p, blockIdx.x / p.cluster, &s_tile, s_sum);
+  const Tile tile = find_tile<kRowsOf>(p, blockIdx.x / p.cluster, &s_tile, s_sum);
   if (!tile.rows || tile.rank == 0) {  // (the same in every CTA of the cluster)
     if (tile.rows) copy_base(p, tile, rank_of_cta);
     cluster_wait();
@@ -263,13 +270,13 @@ __global__ void __launch_bounds__(kThreads, 2) lora_few_kernel(LoraArgs p) {
   const int kb1 = share(p.K / 32, p.cluster, rank_of_cta + 1), kb0 = share(p.K / 32, p.cluster, rank_of_cta) + warp;
   // (A single row is dealt with in f32 -- an instruction for eight rows would be an eighth of its own worth: two lanes on an output up to rank 16, else four, of
   // which each has 8 elements of a piece's 16, 32 or, beyond that, two times 8 of 64.)
-  const bool single = tile.rows == 1, split = single && rank > 32;
+  const bool single = kRowsOf == 1 || tile.rows == 1, split = single && rank > 32;
   const int lanes_log = rank <= 16 ? 1 : 2, lanes = 1 << lanes_log, unit = !single ? 16 : split ? 8 : 64 >> lanes_log;
   const int tiles = (p.N + unit - 1) / unit, nt0 = share(tiles, p.cluster * kWarps, rank_of_cta * kWarps + warp), nt1 = share(tiles, p.cluster * kWarps, rank_of_cta * kWarps + warp + 1);
   const int whole = p.N / unit;  // (a last tile may be cut off)
 
   // ---- the ring: pieces in the order in which they are used below
-  unsigned char* ring = smem + warp * kFewSlots * kFewSlot + lane * 16;
+  unsigned char* ring = smem + warp * kSlots * kSlot + lane * 16;
   const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
   int ask_slot = 0, ask_j0 = kb0 < kb1 ? 0 : rank, ask_kb = kb0, ask_i = 0, ask_nt = nt0, ask_j = 0;
   const size_t eight_a = (size_t)8 * p.K;
@@ -287,8 +294,8 @@ __global__ void __launch_bounds__(kThreads, 2) lora_few_kernel(LoraArgs p) {
   const float* ask_base = p.base + out_row * p.ldb + nt0 * unit + out_at;  // (not looked at without a base)
   float* to = p.C + out_row * p.ldc + nt0 * unit + out_at;
   auto ask = [&]() {
-    const uint32_t to = ring_at + ask_slot * kFewSlot;
-    ask_slot = ask_slot + 1 == kFewSlots ? 0 : ask_slot + 1;
+    const uint32_t to = ring_at + ask_slot * kSlot;
+    ask_slot = ask_slot + 1 == kSlots ? 0 : ask_slot + 1;
     if (ask_j0 < rank) {  // of A
       const uint16_t* from = ask_a + 2 * (ask_j0 / 16 + ask_i) * eight_a;
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n\tcp.async.cg.shared.global [%0+512], [%2], 16;" ::"r"(to), "l"(from), "l"(from + eight_a) : "memory");
@@ -312,7 +319,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_few_kernel(LoraArgs p) {
         const bool cut = ask_nt >= whole;
         const int n = ask_nt * unit + out_at;
         if (single) {
-          if (!cut || n < p.N) copy4(to + 1024, ask_base);
+          if (!cut || n < p.N) copy4(to + 1024 - (kRowsOf == 1 ? lane * 12 : 0), ask_base);
         } else if (vec && !cut) {
           copy16(to + 1024, ask_base);
         } else {
@@ -345,29 +352,32 @@ __global__ void __launch_bounds__(kThreads, 2) lora_few_kernel(LoraArgs p) {
   };
   int slot = 0;
   auto take = [&](uint4& r0, uint4& r1, float4& base) {
-    asm volatile("cp.async.wait_group %0;" ::"n"(kFewSlots - 1) : "memory");
-    r0 = *reinterpret_cast<const uint4*>(ring + slot * kFewSlot);
-    r1 = *reinterpret_cast<const uint4*>(ring + slot * kFewSlot + 512);
-    base = *reinterpret_cast<const float4*>(ring + slot * kFewSlot + 1024);  // (of an output's first piece)
-    slot = slot + 1 == kFewSlots ? 0 : slot + 1;
+    asm volatile("cp.async.wait_group %0;" ::"n"(kSlots - 1) : "memory");
+    r0 = *reinterpret_cast<const uint4*>(ring + slot * kSlot);
+    r1 = *reinterpret_cast<const uint4*>(ring + slot * kSlot + 512);
+    // (of an output's first piece)
+    if (kRowsOf == 1) base.x = *reinterpret_cast<const float*>(ring + slot * kSlot + 1024 - lane * 12);
+    else base = *reinterpret_cast<const float4*>(ring + slot * kSlot + 1024);
+    slot = slot + 1 == kSlots ? 0 : slot + 1;
     ask();
   };
-#pragma unroll
-  for (int i = 0; i < kFewSlots; ++i) ask();
-
-  // ---- u
   const int8_t* x = p.aq + (size_t)(tile.row + min(g, tile.rows - 1)) * p.K + 8 * t;
   const float* xs = p.asc + tile.row + min(g, tile.rows - 1);
+  uint2 v_next = make_uint2(0u, 0u);
+  float s_next = 0.0f;
+  auto values = [&](int kb) {
+    if (kb >= kb1) return;
+    v_next = *reinterpret_cast<const uint2*>(x + kb * 32);
+    s_next = xs[(size_t)kb * p.Mp];
+  };
+  values(kb0);  // (ahead of what fills the queues to memory)
+#pragma unroll
+  for (int i = 0; i < kSlots; ++i) ask();
+
+  // ---- u
   for (int j0 = 0; j0 < rank; j0 += kFewRanks * 16) {
     float acc[kFewRanks][4] = {};  // row g, ranks 2t, 2t + 1, 8 + 2t, 9 + 2t of the tile
-    uint2 v_next = make_uint2(0u, 0u);
-    float s_next = 0.0f;
-    auto values = [&](int kb) {
-      if (kb >= kb1) return;
-      v_next = *reinterpret_cast<const uint2*>(x + kb * 32);
-      s_next = xs[(size_t)kb * p.Mp];
-    };
-    values(kb0);
+    if (j0) values(kb0);
     for (int kb = kb0; kb < kb1; kb += kWarps) {
       const uint4 v = eight_of<kBf16>(v_next);
       const float s0 = s_next;
@@ -389,8 +399,8 @@ __global__ void __launch_bounds__(kThreads, 2) lora_few_kernel(LoraArgs p) {
     }
 #pragma unroll
     for (int i = 0; i < kFewRanks; ++i)
-      if (j0 + i * 16 < rank) {
-        float* to = s_part + (warp * kFewRows + g) * kFewPart + i * 16 + 2 * t;
+      if (j0 + i * 16 < rank && g < kRowsOf) {
+        float* to = s_part + (warp * kRowsOf + g) * kFewPart + i * 16 + 2 * t;
         *reinterpret_cast<float2*>(to) = make_float2(acc[i][0], acc[i][1]);
         *reinterpret_cast<float2*>(to + 8) = make_float2(acc[i][2], acc[i][3]);
       }
@@ -403,10 +413,10 @@ __global__ void __launch_bounds__(kThreads, 2) lora_few_kernel(LoraArgs p) {
       float4 v = *reinterpret_cast<const float4*>(from);
 #pragma unroll
       for (int w = 1; w < kWarps; ++w) {
-        const float4 b = *reinterpret_cast<const float4*>(from + w * kFewRows * kFewPart);
+        const float4 b = *reinterpret_cast<const float4*>(from + w * kRowsOf * kFewPart);
         v.x += b.x; v.y += b.y; v.z += b.z; v.w += b.w;
       }
-      const float* here = s_all + ((size_t)rank_of_cta * kFewRows + row) * (p.R + 8) + j0 + j;
+      const float* here = s_all + ((size_t)rank_of_cta * kRowsOf + row) * (p.R + 8) + j0 + j;
       for (int c = 0; c < p.cluster; ++c) remote_store(at_rank(here, c), v);
     }
     __syncthreads();
@@ -420,7 +430,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_few_kernel(LoraArgs p) {
       float u = 0.0f;
       if (j < rank)
 #pragma unroll 8
-        for (int c = 0; c < p.cluster; ++c) u += s_all[(size_t)c * kFewRows * (p.R + 8) + j];
+        for (int c = 0; c < p.cluster; ++c) u += s_all[(size_t)c * kRowsOf * (p.R + 8) + j];
       s_f[j] = u;
     }
     __syncthreads();
@@ -467,6 +477,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_few_kernel(LoraArgs p) {
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     return;
   }
+  if (kRowsOf == 1) return;
   // ---- the sums of the CTAs in order; a warp per row
   const int chunks = (p.R + 31) / 32;
   if (warp < tile.rows) {
@@ -474,7 +485,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_few_kernel(LoraArgs p) {
       const float* from = s_all + warp * (p.R + 8) + j;
       float u = 0.0f;
 #pragma unroll 8
-      for (int c = 0; c < p.cluster; ++c) u += from[(size_t)c * kFewRows * (p.R + 8)];
+      for (int c = 0; c < p.cluster; ++c) u += from[(size_t)c * kRowsOf * (p.R + 8)];
       return u;
     }, [&](int i, int j, uint16_t v) {
       const Place at = place_of(j, rank);
@@ -929,26 +940,26 @@ extern "C" int izb_lora_add(int dtype, const void* d_A, const void* d_B, int n_a
   IZB_CUDA(cudaGetDevice(&device));
   LoraArgs p = {(const uint16_t*)d_A, (const uint16_t*)d_B, d_ranks, d_seg, d_adapter, d_scales, d_asc, d_base, d_aq, d_C + c_off, n_adapters, R, N, K, T, Mp, n_seg, ldb, ldc, 0};
   cudaStream_t st = (cudaStream_t)stream;
-  const bool bf16 = dtype == IZB_BF16, few = few_rows(T, n_seg);
-  const int64_t tiles = (int64_t)T / (few ? kFewRows : kRows) + n_seg;  // (at most)
+  const bool bf16 = dtype == IZB_BF16, few = few_rows(T, n_seg), one = T <= n_seg;
+  const int64_t tiles = (int64_t)T / (one ? 1 : few ? kFewRows : kRows) + n_seg;  // (at most)
   const int sms = izb_sm_count(device);
   // CTAs per tile.  Few rows: 16 while that leaves the multiprocessors two CTAs at most, else 8.  More rows: as many as fit at once, 8 at most.
-  p.cluster = few && tiles * 16 <= 2 * sms && R <= 128 ? 16 : 8;
+  p.cluster = few && n_seg * 16 <= 2 * sms && R <= 128 ? 16 : 8;
   while (!few && p.cluster > 1 && tiles * p.cluster > 2 * sms) p.cluster /= 2;
   if (tiles * p.cluster > 0x7FFFFFFF) IZB_FAIL(IZB_ERR_LIMIT, "lora_add: %d rows in %d segments", T, n_seg);
   const dim3 grid((unsigned)(tiles * p.cluster));
   if (few) {
-    const size_t smem = few_smem(R, p.cluster);
-    for (auto kernel : {lora_few_kernel<false>, lora_few_kernel<true>}) {
-      static izb_device_once once[2];
-      if (int rc = once[kernel == lora_few_kernel<true>].run(device, [&]() -> int {
-            IZB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(few_smem(kMaxRank, 8) > few_smem(128, 16) ? few_smem(kMaxRank, 8) : few_smem(128, 16))));
-            IZB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-            return IZB_OK;
-          }))
-        return rc;
-    }
-    IZB_LAUNCH("lora_add", st, izb_launch_pdl_cluster(bf16 ? lora_few_kernel<true> : lora_few_kernel<false>, p.cluster, grid, kThreads, smem, st, p));
+    static izb_device_once once[4];
+    void (*const kernels[4])(LoraArgs) = {lora_few_kernel<false, kFewRows>, lora_few_kernel<true, kFewRows>, lora_few_kernel<false, 1>, lora_few_kernel<true, 1>};
+    const int which = (one ? 2 : 0) + bf16;
+    if (int rc = once[which].run(device, [&]() -> int {
+          IZB_CUDA(cudaFuncSetAttribute(kernels[which], cudaFuncAttributeMaxDynamicSharedMemorySize, 200 << 10));
+          IZB_CUDA(cudaFuncSetAttribute(kernels[which], cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+          return IZB_OK;
+        }))
+      return rc;
+    const size_t smem = one ? few_smem<1>(R, p.cluster) : few_smem<kFewRows>(R, p.cluster);
+    IZB_LAUNCH("lora_add", st, izb_launch_pdl_cluster(kernels[which], p.cluster, grid, kThreads, smem, st, p));
     return IZB_OK;
   }
   if (!d_scratch || !izb_aligned(d_scratch, 16)) IZB_FAIL(IZB_ERR_ARG, "lora_add: %d rows in %d segments want %zu bytes of scratch, 16-byte aligned", T, n_seg, izb_lora_scratch(dtype, R, T, n_seg));
