@@ -440,8 +440,57 @@ __global__ void __launch_bounds__(kThreads, kFewBlocks<kRowsOf>) lora_few_kernel
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int e = 0; e < 4; ++e) u[h][e] = *reinterpret_cast<const float2*>(mine + (split ? 32 * h : 0) + 2 * e);
-#pragma unroll 2
-    for (int nt = nt0; nt < nt1; ++nt, to += unit) {
+    int nt = nt0;
+    auto sum_of = [&](const float2 (&v)[2]) {  // over the lanes that share an output (or two)
+      const float a = v[0].x + v[0].y, b = v[1].x + v[1].y;
+      if (split) {
+        float y = a + b;
+        y += __shfl_xor_sync(0xFFFFFFFFu, y, 2);
+        return y + __shfl_xor_sync(0xFFFFFFFFu, y, 1);
+      }
+      const float y = (upper ? b : a) + __shfl_xor_sync(0xFFFFFFFFu, upper ? a : b, lanes >> 1);
+      return lanes == 4 ? y + __shfl_xor_sync(0xFFFFFFFFu, y, 1) : y;
+    };
+    auto add = [&](float2 (&v)[2], const uint4 (&r)[2]) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t w[4] = {r[h].x, r[h].y, r[h].z, r[h].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[h] = fma2(two_values<kBf16>(w[e]), u[h][e], v[h]);
+      }
+    };
+    // Whole units of one piece each, which are nearly all there are: the ring's upkeep is a few additions (take() and ask() are four times as much)
+    if (rank <= 64 && ask_nt < nt1) {
+      const int j0 = (lane & (lanes - 1)) * 8, j1 = split ? j0 + 32 : j0, bytes0 = j0 < rank ? 16 : 0, bytes1 = j1 < rank ? 16 : 0;
+      const uint16_t *from0 = ask_b + (bytes0 ? j0 : 0), *from1 = ask_b + step_b + (bytes1 ? j1 : 0);
+      const float* base_from = ask_base;
+      const bool with_base = p.base && mine_has;
+      const int ask_end = min(nt1, whole);
+      // (while what is asked for is whole, what is taken is)
+      for (; ask_nt < ask_end; ++ask_nt, ++nt) {
+        copies_there<kSlots - 1>();
+        const unsigned char* here = ring + slot * kSlot;
+        const uint4 r[2] = {*reinterpret_cast<const uint4*>(here), *reinterpret_cast<const uint4*>(here + 512)};
+        const float base = with_base ? *reinterpret_cast<const float*>(here + 1024 - (kRowsOf == 1 ? lane * 12 : 0)) : 0.0f;
+        const uint32_t at = ring_at + slot * kSlot;  // (the slot that has been read is the next one to fill)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %3;\n\tcp.async.cg.shared.global [%0+512], [%2], 16, %4;" ::"r"(at), "l"(from0), "l"(from1), "r"(bytes0), "r"(bytes1) : "memory");
+        if (with_base) copy4(at + 1024 - (kRowsOf == 1 ? lane * 12 : 0), base_from);
+        copies_begun();
+        from0 += unit_b;
+        from1 += unit_b;
+        base_from += unit;
+        slot = slot + 1 == kSlots ? 0 : slot + 1;
+        float2 v[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+        add(v, r);
+        const float y = sum_of(v);
+        if (mine_has) *to = fmaf(tile.scale, y, base);
+        to += unit;
+      }
+      ask_slot = slot;
+      ask_b += unit_b * (size_t)(nt - nt0);
+      ask_base += (size_t)unit * (nt - nt0);
+    }
+    for (; nt < nt1; ++nt, to += unit) {
       float base = 0.0f;
       float2 v[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
       for (int j = 0; j < rank; j += 64) {
@@ -455,23 +504,9 @@ __global__ void __launch_bounds__(kThreads, kFewBlocks<kRowsOf>) lora_few_kernel
 #pragma unroll
             for (int e = 0; e < 4; ++e) u[h][e] = *reinterpret_cast<const float2*>(mine + j + 32 * h + 2 * e);
         }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t w[4] = {r[h].x, r[h].y, r[h].z, r[h].w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[h] = fma2(two_values<kBf16>(w[e]), u[h][e], v[h]);
-        }
+        add(v, r);
       }
-      const float a = v[0].x + v[0].y, b = v[1].x + v[1].y;
-      float y;
-      if (split) {
-        y = a + b;
-        y += __shfl_xor_sync(0xFFFFFFFFu, y, 2);
-        y += __shfl_xor_sync(0xFFFFFFFFu, y, 1);
-      } else {
-        y = (upper ? b : a) + __shfl_xor_sync(0xFFFFFFFFu, upper ? a : b, lanes >> 1);
-        if (lanes == 4) y += __shfl_xor_sync(0xFFFFFFFFu, y, 1);
-      }
+      const float y = sum_of(v);
       if (mine_has && (nt < whole || nt * unit + out_at < p.N)) *to = fmaf(tile.scale, y, base);
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
