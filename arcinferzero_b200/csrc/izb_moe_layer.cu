@@ -21,7 +21,7 @@
 namespace {
 
 constexpr int kMaxTokens = 32, kMaxPairs = 512, kMaxExperts = 512, kMaxChoices = 32;
-constexpr int kUpWarps = 16, kSplitK = 8;  // first kernel: two groups of 16 channels x eight parts of K
+constexpr int kUpWarps = 8, kSplitK = 4;   // first kernel: two groups of 16 channels x four parts of K
 constexpr int kDownWarps = 16;
 constexpr int kGroup = 8;                  // tokens of an expert that are dealt with in one go
 constexpr uint32_t kMagic = 0x4B400000u;  // 1.5 * 2^23: accumulators start there and are f32 numbers as they are (|sum| < 2^22)
@@ -152,8 +152,39 @@ __device__ __forceinline__ void mma(int (&d)[4], uint32_t a0, uint32_t a1, uint3
     asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-struct Scales {  // of rows g, g + 8 and blocks 2t, 2t + 1
-  float s[2][2], m[2][2];
+// f32 pairs (blocks 2t and 2t + 1): two IEEE operations per instruction
+typedef unsigned long long f2;
+__device__ __forceinline__ f2 f2_of(float x, float y) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 f2_parts(f2 a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
+  return r;
+}
+__device__ __forceinline__ f2 f2_add(f2 a, f2 b) {
+  f2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f2 f2_mul(f2 a, f2 b) {
+  f2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f2 f2_fma(f2 a, f2 b, f2 c) {
+  f2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+// two accumulators as the numbers they are
+__device__ __forceinline__ f2 numbers(int a, int b) {
+  return f2_add(f2_of(__int_as_float(a), __int_as_float(b)), f2_of(-__uint_as_float(kMagic), -__uint_as_float(kMagic)));
+}
+struct Scales {  // of rows g, g + 8 for blocks 2t, 2t + 1; mins with their sign changed
+  f2 s[2], m[2];
 };
 template <int QT>
 struct Raw;
@@ -189,11 +220,10 @@ struct Raw<IZB_Q4_K> {
       const uint32_t a = h[r].y >> sh, b = h[r].z >> sh, c = h[r].w >> sh;  // two blocks side by side
       const uint32_t sc = t < 2 ? a & 0x3F3Fu : (c & 0x0F0Fu) | ((a >> 2) & 0x3030u), mn = t < 2 ? b & 0x3F3Fu : ((c >> 4) & 0x0F0Fu) | ((b >> 2) & 0x3030u);
       // (a byte under the exponent of 2^23 is the number 2^23 + byte, and d * that - d * 2^23 is rounded once: no conversions)
-      const float d = half_bits_to_float(h[r].x & 0xFFFFu), dm = half_bits_to_float(h[r].x >> 16), d0 = -8388608.0f * d, m0 = -8388608.0f * dm;
-      o.s[r][0] = fmaf(d, __uint_as_float(__byte_perm(sc, 0x4B000000u, 0x7440)), d0);
-      o.s[r][1] = fmaf(d * 0.0625f, __uint_as_float(__byte_perm(sc, 0x4B000000u, 0x7441)), d0 * 0.0625f);
-      o.m[r][0] = fmaf(dm, __uint_as_float(__byte_perm(mn, 0x4B000000u, 0x7440)), m0);
-      o.m[r][1] = fmaf(dm, __uint_as_float(__byte_perm(mn, 0x4B000000u, 0x7441)), m0);
+      const float d = half_bits_to_float(h[r].x & 0xFFFFu), dm = -half_bits_to_float(h[r].x >> 16);
+      const f2 dd = f2_of(d, d * 0.0625f), mm = f2_of(dm, dm), big = f2_of(-8388608.0f, -8388608.0f);
+      o.s[r] = f2_fma(dd, f2_of(__uint_as_float(__byte_perm(sc, 0x4B000000u, 0x7440)), __uint_as_float(__byte_perm(sc, 0x4B000000u, 0x7441))), f2_mul(dd, big));
+      o.m[r] = f2_fma(mm, f2_of(__uint_as_float(__byte_perm(mn, 0x4B000000u, 0x7440)), __uint_as_float(__byte_perm(mn, 0x4B000000u, 0x7441))), f2_mul(mm, big));
     }
   }
 };
@@ -220,13 +250,10 @@ struct Raw<IZB_Q8_0> {
   __device__ __forceinline__ void scales(Scales& o, int) const {
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      o.s[r][0] = half_bits_to_float(h[r] & 0xFFFFu);
-      o.s[r][1] = half_bits_to_float(h[r] >> 16);
+      o.s[r] = f2_of(half_bits_to_float(h[r] & 0xFFFFu), half_bits_to_float(h[r] >> 16));
     }
   }
 };
-__device__ __forceinline__ float number(int d) { return __int_as_float(d) - __uint_as_float(kMagic); }
-
 // A warp's copies of pieces into its ring.
 template <int QT>
 struct Copier {
@@ -256,14 +283,14 @@ __device__ __forceinline__ void copies_there() {
 }
 
 // ---------------------------------------------------------------------------------------------- gate, up, SwiGLU
-// A CTA takes 32 channels of one expert at a time (one block of h); a warp 16 of them, gate and up, for every eighth superblock.
+// A CTA takes 32 channels of one expert at a time (one block of h); a warp 16 of them, gate and up, for every fourth superblock.
 template <int QT>
 struct Up {
   static constexpr int kSlots = QT == IZB_Q4_K ? 2 : 1, kSlot = 2 * Copier<QT>::kTile;
   static constexpr size_t kSums = 2 * kUpWarps * kGroup * 32 * sizeof(float), kSmem = kSums + (size_t)kUpWarps * kSlots * kSlot;
 };
 template <int QT>
-__global__ void __launch_bounds__(kUpWarps * 32, 1) moe_layer_up_kernel(MoeArgs p) {
+__global__ void __launch_bounds__(kUpWarps * 32, 2) moe_layer_up_kernel(MoeArgs p) {
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ Routed s;
   constexpr int kSlots = Up<QT>::kSlots, kSlot = Up<QT>::kSlot;
@@ -354,22 +381,23 @@ __global__ void __launch_bounds__(kUpWarps * 32, 1) moe_layer_up_kernel(MoeArgs 
         int dg[4], du[4];
         wg.dots(dg, x_now, g);
         wu.dots(du, x_now, g);
-        float v[4];  // gate row g, g + 8, up row g, g + 8
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          v[r] = fmaf(number(dg[2 * r]) * cg.s[r][0], s0, number(dg[2 * r + 1]) * cg.s[r][1] * s1);
-          v[2 + r] = fmaf(number(du[2 * r]) * cu.s[r][0], s0, number(du[2 * r + 1]) * cu.s[r][1] * s1);
-        }
+        const f2 ss = f2_of(s0, s1);
+        f2 sums = 0;
         if (Raw<QT>::kMin) {
           int sum = __dp4a((int)x_now.x, 0x01010101, __dp4a((int)x_now.y, 0x01010101, 0));  // of block g
           sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
           sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
-          const float x0 = (float)__shfl_sync(0xFFFFFFFFu, sum, 8 * t) * s0, x1 = (float)__shfl_sync(0xFFFFFFFFu, sum, 8 * t + 4) * s1;
+          sums = f2_mul(f2_of((float)__shfl_sync(0xFFFFFFFFu, sum, 8 * t), (float)__shfl_sync(0xFFFFFFFFu, sum, 8 * t + 4)), ss);
+        }
+        float v[4];  // gate row g, g + 8, up row g, g + 8
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            v[r] = fmaf(-cg.m[r][0], x0, fmaf(-cg.m[r][1], x1, v[r]));
-            v[2 + r] = fmaf(-cu.m[r][0], x0, fmaf(-cu.m[r][1], x1, v[2 + r]));
-          }
+        for (int r = 0; r < 4; ++r) {
+          const Scales& c = r < 2 ? cg : cu;
+          const int* d = r < 2 ? dg : du;
+          f2 q = f2_mul(f2_mul(numbers(d[2 * (r & 1)], d[2 * (r & 1) + 1]), c.s[r & 1]), ss);
+          if (Raw<QT>::kMin) q = f2_fma(c.m[r & 1], sums, q);
+          const float2 both = f2_parts(q);
+          v[r] = both.x + both.y;
         }
         // the quad's sums: lane t keeps v[t]
         const bool odd = t & 1, high = t & 2;
@@ -438,6 +466,13 @@ __global__ void __launch_bounds__(kDownWarps * 32, 1) moe_layer_down_kernel(MoeA
   pdl_launch_next();
   const int splits_log = p.splits - 1, warps_log = __ffs(warps) - 1, items = route_all(p, s) << splits_log, sbs = p.F / 256, per = p.F / 32;  // (one or two splits)
 
+  // what the combine adds to (written before this call's first kernel, so it may be read here)
+  const int first_at = min((int)threadIdx.x >> 4, p.T - 1) * p.E + blockIdx.x * 16 + (threadIdx.x & 15);
+  float base = 0.0f, shared = 0.0f;
+  auto shared_of = [&](int token, int at) { return p.sh[at] / (1.0f + expf(-p.logits[(size_t)token * p.ldl + p.NE])); };
+  if (p.x) base = p.x[first_at];
+  if (p.sh) shared = shared_of(min((int)threadIdx.x >> 4, p.T - 1), first_at);
+
   // A place in a warp's work: 16 outputs, an item (an expert's tokens and a part of F: parts of unlike lengths go round among the warps), a superblock.
   struct Place {
     int n0, item, sb, end, k;
@@ -476,7 +511,7 @@ __global__ void __launch_bounds__(kDownWarps * 32, 1) moe_layer_down_kernel(MoeA
   pdl_wait();
 
   uint2 x[3];
-  float2 hs, hm;
+  f2 hs, hm;
   int pair = 0;
   auto values = [&](const Place& w, int token) {
     pair = pair_of(p, s, token, s.list[w.item >> splits_log]);
@@ -485,8 +520,8 @@ __global__ void __launch_bounds__(kDownWarps * 32, 1) moe_layer_down_kernel(MoeA
     x[1] = *reinterpret_cast<const uint2*>(hq + p.F);
     x[2] = *reinterpret_cast<const uint2*>(hq + 2 * p.F);
     const int at = pair * per + w.sb * 8 + 2 * t;
-    hs = *reinterpret_cast<const float2*>(p.hs + at);
-    if (Raw<QT>::kMin) hm = *reinterpret_cast<const float2*>(p.hsum + at);
+    hs = *reinterpret_cast<const f2*>(p.hs + at);
+    if (Raw<QT>::kMin) hm = *reinterpret_cast<const f2*>(p.hsum + at);
   };
   if (now.n0 < p.E) values(now, __ffs(s.group[now.item >> splits_log]) - 1);
   for (int n0 = blockIdx.x * 16, slot = 0; n0 < p.E; n0 += gridDim.x * 16) {
@@ -509,18 +544,19 @@ __global__ void __launch_bounds__(kDownWarps * 32, 1) moe_layer_down_kernel(MoeA
         w.dots(d1, x[0], g);
         w.dots(d2, x[1], g);
         w.dots(d3, x[2], g);
-        const float2 hs_now = hs, hm_now = hm;
+        const f2 hs_now = hs, hm_now = hm;
         const int pair_now = pair;
         if (left) values(here, __ffs(left) - 1);
         else if (now.n0 < p.E) values(now, __ffs(s.group[now.item >> splits_log]) - 1);
         float v[2];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          float q[2];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) q[i] = fmaf(number(d1[2 * r + i]), 65536.0f, fmaf(number(d2[2 * r + i]), 256.0f, number(d3[2 * r + i]))) * c.s[r][i];
-          v[r] = fmaf(q[0], hs_now.x, q[1] * hs_now.y);
-          if (Raw<QT>::kMin) v[r] = fmaf(-c.m[r][0], hm_now.x, fmaf(-c.m[r][1], hm_now.y, v[r]));
+          f2 q = f2_fma(numbers(d2[2 * r], d2[2 * r + 1]), f2_of(256.0f, 256.0f), numbers(d3[2 * r], d3[2 * r + 1]));
+          q = f2_fma(numbers(d1[2 * r], d1[2 * r + 1]), f2_of(65536.0f, 65536.0f), q);
+          q = f2_mul(f2_mul(q, c.s[r]), hs_now);
+          if (Raw<QT>::kMin) q = f2_fma(c.m[r], hm_now, q);
+          const float2 both = f2_parts(q);
+          v[r] = both.x + both.y;
         }
         float a = (t & 1 ? v[1] : v[0]) + __shfl_xor_sync(0xFFFFFFFFu, t & 1 ? v[0] : v[1], 1);
         a += __shfl_xor_sync(0xFFFFFFFFu, a, 2);
@@ -533,7 +569,10 @@ __global__ void __launch_bounds__(kDownWarps * 32, 1) moe_layer_down_kernel(MoeA
     __syncthreads();
     for (int i = threadIdx.x; i < p.T * 16; i += blockDim.x) {
       const int token = i >> 4, at = token * p.E + n0 + (i & 15), pr0 = token * p.NU;
-      const float base = p.x ? p.x[at] : 0.0f;
+      if (i >= (int)blockDim.x || n0 != (int)blockIdx.x * 16) {
+        if (p.x) base = p.x[at];
+        if (p.sh) shared = shared_of(token, at);
+      }
       float v = 0.0f;
 #pragma unroll 4
       for (int k = 0; k < p.NU; ++k) {
@@ -541,7 +580,7 @@ __global__ void __launch_bounds__(kDownWarps * 32, 1) moe_layer_down_kernel(MoeA
         const float sum = splits_log ? y[0] + y[16] : y[0], next = fmaf(s.wt[pr0 + k], sum, v);
         if (s.id[pr0 + k] >= 0) v = next;
       }
-      if (p.sh) v = fmaf(p.sh[at], 1.0f / (1.0f + expf(-p.logits[(size_t)token * p.ldl + p.NE])), v);
+      if (p.sh) v += shared;
       p.out[at] = p.x ? base + v : v;
     }
     __syncthreads();
@@ -591,7 +630,7 @@ extern "C" int izb_moe_layer(const izb_weight* wg, const izb_weight* wu, const i
   p.joined = wg->gu32; p.gate_row = wg->row_bytes; p.down_row = wd->row_bytes;
   p.splits = F >= 512 ? 2 : 1;
   const int sms = izb_sm_count(wg->device), units = (int)(pairs < (size_t)wg->n_mats ? pairs : wg->n_mats) * (F / 32);
-  const int up_grid = units < sms ? units : sms;
+  const int up_grid = units < 2 * sms ? units : 2 * sms;
   // the second kernel: a CTA of 16 warps per multiprocessor, or two of 8 where one round of the former does not do
   const int tiles = E / 16, down_warps = tiles <= sms ? kDownWarps : kDownWarps / 2, most = tiles <= sms ? sms : 2 * sms;
   const int down_grid = tiles < most ? tiles : most;
