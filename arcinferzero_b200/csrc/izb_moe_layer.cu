@@ -71,23 +71,25 @@ __device__ __forceinline__ void route_token(const MoeArgs& p, int token, Routed&
       if (key[i] > best) { best = key[i]; at = i; }
   };
   rescan();
-  float top = 0.0f, denom = 0.0f, mine = 0.0f;
+  uint32_t mine_key = 0u;
   int id = 0;
   for (int k = 0; k < p.NU; ++k) {
     const uint32_t win = __reduce_max_sync(0xFFFFFFFFu, best);
-    const int e = (int)__reduce_min_sync(0xFFFFFFFFu, best == win ? (uint32_t)(at * 32 + lane) : 0xFFFFu);
-    if ((e & 31) == lane) {
+    const uint32_t who = __ballot_sync(0xFFFFFFFFu, best == win);
+    // (one lane as a rule: the minimum over ids is only looked for where several hold the same logit)
+    const int e = who & (who - 1) ? (int)__reduce_min_sync(0xFFFFFFFFu, best == win ? (uint32_t)(at * 32 + lane) : 0xFFFFu)
+                                  : __shfl_sync(0xFFFFFFFFu, at * 32 + lane, __ffs(who) - 1);
 #pragma unroll
-      for (int i = 0; i < kPer; ++i)
-        if (i == (e >> 5)) key[i] = 0u;
-      rescan();
-    }
-    const float l = __uint_as_float((win & 0x80000000u) ? (win & 0x7FFFFFFFu) : ~win);
-    if (k == 0) top = l;
-    const float q = expf(l - top);
-    denom += q;
-    if (lane == k) { mine = q; id = e; }
+    for (int i = 0; i < kPer; ++i)
+      if (i * 32 + lane == e) key[i] = 0u;
+    if ((e & 31) == lane) rescan();
+    if (lane == k) { mine_key = win; id = e; }
   }
+  // p_k = exp(l_k - l_0), their sum in choice order
+  const float l = __uint_as_float((mine_key & 0x80000000u) ? (mine_key & 0x7FFFFFFFu) : ~mine_key);
+  const float mine = expf(l - __shfl_sync(0xFFFFFFFFu, l, 0));
+  float denom = 0.0f;
+  for (int k = 0; k < p.NU; ++k) denom += __shfl_sync(0xFFFFFFFFu, mine, k);
   if (lane < p.NU) {
     const int e = id - p.e0;
     const bool here = e >= 0 && e < p.n_mats;
@@ -97,7 +99,7 @@ __device__ __forceinline__ void route_token(const MoeArgs& p, int token, Routed&
   }
 }
 // All tokens; the length of the list.  Every thread of the CTA calls it.
-__device__ int route_all(const MoeArgs& p, Routed& s) {
+__device__ __forceinline__ int route_all(const MoeArgs& p, Routed& s) {
   const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5, lane = threadIdx.x & 31;
   for (int i = threadIdx.x; i < kMaxExperts; i += blockDim.x) s.tokens[i] = 0u;
   __syncthreads();
@@ -289,6 +291,37 @@ struct Up {
   static constexpr int kSlots = QT == IZB_Q4_K ? 2 : 1, kSlot = 2 * Copier<QT>::kTile;
   static constexpr size_t kSums = 2 * kUpWarps * kGroup * 32 * sizeof(float), kSmem = kSums + (size_t)kUpWarps * kSlots * kSlot;
 };
+// The sums of a unit: a warp per token, channel f0 + lane.
+__device__ __forceinline__ void up_epilogue(const MoeArgs& p, const Routed& s, const float (*sums)[kGroup][32], int entry, int f0, uint32_t tokens) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, per = p.F / 32, live = min(kSplitK, p.E / 256);
+  for (int i = 0; i < warp; ++i) tokens &= tokens - 1;
+  const int pair = pair_of(p, s, __ffs(tokens) - 1, s.list[entry]);
+  float gate = 0.0f, up = 0.0f;
+#pragma unroll
+  for (int k = 0; k < kSplitK; ++k) {
+    if (k >= live) break;
+    const float* from = sums[(lane >> 4) * kSplitK + k][warp];
+    gate += from[lane & 15];
+    up += from[16 + (lane & 15)];
+  }
+  const float h = gate / (1.0f + expf(-gate)) * up;
+  const uint32_t most = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(h) & 0x7FFFFFFFu);  // (a NaN is above all numbers here)
+  const int ex = max((int)(most >> 23), 1) - 127;                                           // |h| < 2^(ex + 1)
+  const bool none = most >= 0x7F800000u;
+  const int up1 = min(21 - ex, 100);
+  const int Q = none ? 0 : __float2int_rn(h * __int_as_float((up1 + 127) << 23) * __int_as_float((21 - ex - up1 + 127) << 23));
+  const int d3 = (int8_t)Q, q1 = (Q - d3) >> 8, d2 = (int8_t)q1, d1 = (q1 - d2) >> 8;
+  const int sum = __reduce_add_sync(0xFFFFFFFFu, Q);
+  int8_t* hq = p.hq + (size_t)pair * 3 * p.F + f0 + lane;
+  hq[0] = (int8_t)d1;
+  hq[p.F] = (int8_t)d2;
+  hq[2 * p.F] = (int8_t)d3;
+  if (lane == 0) {
+    const float unit_of = none ? __int_as_float(0x7FC00000) : ldexpf(1.0f, ex - 21);
+    p.hs[(size_t)pair * per + f0 / 32] = unit_of;
+    p.hsum[(size_t)pair * per + f0 / 32] = unit_of * (float)sum;
+  }
+}
 template <int QT>
 __global__ void __launch_bounds__(kUpWarps * 32, 2) moe_layer_up_kernel(MoeArgs p) {
   extern __shared__ __align__(16) unsigned char smem[];
@@ -301,7 +334,7 @@ __global__ void __launch_bounds__(kUpWarps * 32, 2) moe_layer_up_kernel(MoeArgs 
   const Copier<QT> copier(p.gate_row, lane);
   pdl_wait();
   pdl_launch_next();
-  const int per = p.F / 32, sbs = p.E / 256, entries = route_all(p, s), live = min(kSplitK, sbs);
+  const int sbs = p.E / 256, entries = route_all(p, s);
 
   // A unit is an entry of the list and a block of 32 channels; a CTA takes every gridDim.x-th.
   struct Unit {
@@ -410,38 +443,7 @@ __global__ void __launch_bounds__(kUpWarps * 32, 2) moe_layer_up_kernel(MoeArgs 
     }
     // One barrier per unit: the sums of the unit before last have been read before a warp comes to the barrier of the last one.
     __syncthreads();
-    // a warp per token: channel f0 + lane
-    const int n_tok = __popc(tokens), f0 = unit.f0;
-    if (warp < n_tok) {
-      uint32_t left = tokens;
-      for (int i = 0; i < warp; ++i) left &= left - 1;
-      const int pair = pair_of(p, s, __ffs(left) - 1, s.list[unit.entry]);
-      float gate = 0.0f, up = 0.0f;
-#pragma unroll
-      for (int k = 0; k < kSplitK; ++k) {
-        if (k >= live) break;
-        const float* from = s_sum[buf][(lane >> 4) * kSplitK + k][warp];
-        gate += from[lane & 15];
-        up += from[16 + (lane & 15)];
-      }
-      const float h = gate / (1.0f + expf(-gate)) * up;
-      const uint32_t most = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(h) & 0x7FFFFFFFu);  // (a NaN is above all numbers here)
-      const int ex = max((int)(most >> 23), 1) - 127;                                           // |h| < 2^(ex + 1)
-      const bool none = most >= 0x7F800000u;
-      const int up1 = min(21 - ex, 100);
-      const int Q = none ? 0 : __float2int_rn(h * __int_as_float((up1 + 127) << 23) * __int_as_float((21 - ex - up1 + 127) << 23));
-      const int d3 = (int8_t)Q, q1 = (Q - d3) >> 8, d2 = (int8_t)q1, d1 = (q1 - d2) >> 8;
-      int8_t* hq = p.hq + (size_t)pair * 3 * p.F + f0 + lane;
-      hq[0] = (int8_t)d1;
-      hq[p.F] = (int8_t)d2;
-      hq[2 * p.F] = (int8_t)d3;
-      const int sum = __reduce_add_sync(0xFFFFFFFFu, Q);
-      if (lane == 0) {
-        const float unit_of = none ? __int_as_float(0x7FC00000) : ldexpf(1.0f, ex - 21);
-        p.hs[(size_t)pair * per + f0 / 32] = unit_of;
-        p.hsum[(size_t)pair * per + f0 / 32] = unit_of * (float)sum;
-      }
-    }
+    if (warp < __popc(tokens)) up_epilogue(p, s, s_sum[buf], unit.entry, unit.f0, tokens);
   }
 }
 
@@ -453,6 +455,23 @@ struct Down {
   static constexpr int kSlots = QT == IZB_Q4_K ? 3 : 2, kSlot = Copier<QT>::kTile;
   static size_t smem(int warps, size_t pairs, int splits) { return pairs * splits * 16 * sizeof(float) + (size_t)warps * kSlots * kSlot; }
 };
+// 16 outputs of all tokens.  `base`: what a thread adds in its first output of the CTA's first 16, asked for ahead.
+__device__ __forceinline__ void down_combine(const MoeArgs& p, const Routed& s, const float* s_y, int n0, bool ahead, float base) {
+  const int splits_log = p.splits - 1;
+  for (int i = threadIdx.x; i < p.T * 16; i += blockDim.x) {
+    const int token = i >> 4, at = token * p.E + n0 + (i & 15), pr0 = token * p.NU;
+    if (p.x && (!ahead || i >= (int)blockDim.x)) base = p.x[at];
+    float v = 0.0f;
+#pragma unroll 4
+    for (int k = 0; k < p.NU; ++k) {
+      const float* y = s_y + ((pr0 + k) << splits_log) * 16 + (i & 15);
+      const float sum = splits_log ? y[0] + y[16] : y[0], next = fmaf(s.wt[pr0 + k], sum, v);
+      if (s.id[pr0 + k] >= 0) v = next;
+    }
+    if (p.sh) v = fmaf(p.sh[at], 1.0f / (1.0f + expf(-p.logits[(size_t)token * p.ldl + p.NE])), v);
+    p.out[at] = p.x ? base + v : v;
+  }
+}
 template <int QT>
 __global__ void __launch_bounds__(kDownWarps * 32, 1) moe_layer_down_kernel(MoeArgs p) {
   extern __shared__ __align__(16) unsigned char smem[];
@@ -467,11 +486,8 @@ __global__ void __launch_bounds__(kDownWarps * 32, 1) moe_layer_down_kernel(MoeA
   const int splits_log = p.splits - 1, warps_log = __ffs(warps) - 1, items = route_all(p, s) << splits_log, sbs = p.F / 256, per = p.F / 32;  // (one or two splits)
 
   // what the combine adds to (written before this call's first kernel, so it may be read here)
-  const int first_at = min((int)threadIdx.x >> 4, p.T - 1) * p.E + blockIdx.x * 16 + (threadIdx.x & 15);
-  float base = 0.0f, shared = 0.0f;
-  auto shared_of = [&](int token, int at) { return p.sh[at] / (1.0f + expf(-p.logits[(size_t)token * p.ldl + p.NE])); };
-  if (p.x) base = p.x[first_at];
-  if (p.sh) shared = shared_of(min((int)threadIdx.x >> 4, p.T - 1), first_at);
+  float base = 0.0f;
+  if (p.x) base = p.x[min((int)threadIdx.x >> 4, p.T - 1) * p.E + blockIdx.x * 16 + (threadIdx.x & 15)];
 
   // A place in a warp's work: 16 outputs, an item (an expert's tokens and a part of F: parts of unlike lengths go round among the warps), a superblock.
   struct Place {
@@ -567,22 +583,7 @@ __global__ void __launch_bounds__(kDownWarps * 32, 1) moe_layer_down_kernel(MoeA
       }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < p.T * 16; i += blockDim.x) {
-      const int token = i >> 4, at = token * p.E + n0 + (i & 15), pr0 = token * p.NU;
-      if (i >= (int)blockDim.x || n0 != (int)blockIdx.x * 16) {
-        if (p.x) base = p.x[at];
-        if (p.sh) shared = shared_of(token, at);
-      }
-      float v = 0.0f;
-#pragma unroll 4
-      for (int k = 0; k < p.NU; ++k) {
-        const float* y = s_y + ((pr0 + k) << splits_log) * 16 + (i & 15);
-        const float sum = splits_log ? y[0] + y[16] : y[0], next = fmaf(s.wt[pr0 + k], sum, v);
-        if (s.id[pr0 + k] >= 0) v = next;
-      }
-      if (p.sh) v += shared;
-      p.out[at] = p.x ? base + v : v;
-    }
+    down_combine(p, s, s_y, n0, n0 == (int)blockIdx.x * 16, base);
     __syncthreads();
   }
 }
