@@ -205,15 +205,11 @@ struct Raw<IZB_Q4_K> {
       for (int c = 0; c < 4; ++c) q[r][c] = *reinterpret_cast<const uint2*>(row + 16 + 32 * c + 8 * t);
     }
   }
-  // high nibbles are multiplied where they are, as 16 q: their scale is a 16th
-  __device__ __forceinline__ void dots(int (&d)[4], uint2 x, int g) const {
-    d[0] = d[1] = d[2] = d[3] = (int)kMagic;
-#pragma unroll
-    for (int b = 0; b < 8; ++b) {
-      const uint2 u = q[0][b >> 1], v = q[1][b >> 1];
-      const uint32_t m = b & 1 ? 0xF0F0F0F0u : 0x0F0F0F0Fu;
-      mma<true>(d, u.x & m, v.x & m, u.y & m, v.y & m, g == b ? x.x : 0u, g == b ? x.y : 0u);
-    }
+  // block b's rows; high nibbles are multiplied where they are, as 16 q: their scale is a 16th
+  __device__ __forceinline__ uint4 block(int b) const {
+    const uint2 u = q[0][b >> 1], v = q[1][b >> 1];
+    const uint32_t m = b & 1 ? 0xF0F0F0F0u : 0x0F0F0F0Fu;
+    return make_uint4(u.x & m, v.x & m, u.y & m, v.y & m);
   }
   __device__ __forceinline__ void scales(Scales& o, int t) const {
     const int sh = 16 * (t & 1);
@@ -244,11 +240,7 @@ struct Raw<IZB_Q8_0> {
       for (int c = 0; c < 8; ++c) q[r][c] = *reinterpret_cast<const uint2*>(row + 16 + 32 * c + 8 * t);
     }
   }
-  __device__ __forceinline__ void dots(int (&d)[4], uint2 x, int g) const {
-    d[0] = d[1] = d[2] = d[3] = (int)kMagic;
-#pragma unroll
-    for (int b = 0; b < 8; ++b) mma<false>(d, q[0][b].x, q[1][b].x, q[0][b].y, q[1][b].y, g == b ? x.x : 0u, g == b ? x.y : 0u);
-  }
+  __device__ __forceinline__ uint4 block(int b) const { return make_uint4(q[0][b].x, q[1][b].x, q[0][b].y, q[1][b].y); }
   __device__ __forceinline__ void scales(Scales& o, int) const {
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
@@ -256,6 +248,25 @@ struct Raw<IZB_Q8_0> {
     }
   }
 };
+// The sums of 16 rows x 8 blocks: kW pieces of weights against kX rows of values (one of the two is 1).  A block's operands are made once for all of them.
+template <int kW, int kX, int QT>
+__device__ __forceinline__ void dots(int (&d)[kW * kX][4], const Raw<QT>* const (&w)[kW], const uint2 (&x)[kX], int g) {
+#pragma unroll
+  for (int i = 0; i < kW * kX; ++i) d[i][0] = d[i][1] = d[i][2] = d[i][3] = (int)kMagic;
+#pragma unroll
+  for (int b = 0; b < 8; ++b) {
+    uint2 v[kX];
+#pragma unroll
+    for (int i = 0; i < kX; ++i) v[i] = make_uint2(g == b ? x[i].x : 0u, g == b ? x[i].y : 0u);
+#pragma unroll
+    for (int j = 0; j < kW; ++j) {
+      const uint4 a = w[j]->block(b);
+#pragma unroll
+      for (int i = 0; i < kX; ++i) mma<Raw<QT>::kMin>(d[j * kX + i], a.x, a.y, a.z, a.w, v[i].x, v[i].y);
+    }
+  }
+}
+
 // A warp's copies of pieces into its ring.
 template <int QT>
 struct Copier {
@@ -411,9 +422,10 @@ __global__ void __launch_bounds__(kUpWarps * 32, 2) moe_layer_up_kernel(MoeArgs 
           xs[0] = scale(token, 0);
           xs[1] = scale(token, 1);
         }
-        int dg[4], du[4];
-        wg.dots(dg, x_now, g);
-        wu.dots(du, x_now, g);
+        int d[2][4];
+        const Raw<QT>* const both_weights[2] = {&wg, &wu};
+        const uint2 values_now[1] = {x_now};
+        dots(d, both_weights, values_now, g);
         const f2 ss = f2_of(s0, s1);
         f2 sums = 0;
         if (Raw<QT>::kMin) {
@@ -426,8 +438,7 @@ __global__ void __launch_bounds__(kUpWarps * 32, 2) moe_layer_up_kernel(MoeArgs 
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const Scales& c = r < 2 ? cg : cu;
-          const int* d = r < 2 ? dg : du;
-          f2 q = f2_mul(f2_mul(numbers(d[2 * (r & 1)], d[2 * (r & 1) + 1]), c.s[r & 1]), ss);
+          f2 q = f2_mul(f2_mul(numbers(d[r >> 1][2 * (r & 1)], d[r >> 1][2 * (r & 1) + 1]), c.s[r & 1]), ss);
           if (Raw<QT>::kMin) q = f2_fma(c.m[r & 1], sums, q);
           const float2 both = f2_parts(q);
           v[r] = both.x + both.y;
@@ -556,10 +567,9 @@ __global__ void __launch_bounds__(kDownWarps * 32, 1) moe_layer_down_kernel(MoeA
       const bool first = here.sb == (here.k ? sbs >> 1 : 0);
       while (left) {
         left &= left - 1;
-        int d1[4], d2[4], d3[4];
-        w.dots(d1, x[0], g);
-        w.dots(d2, x[1], g);
-        w.dots(d3, x[2], g);
+        int d[3][4];
+        const Raw<QT>* const weights[1] = {&w};
+        dots(d, weights, x, g);
         const f2 hs_now = hs, hm_now = hm;
         const int pair_now = pair;
         if (left) values(here, __ffs(left) - 1);
@@ -567,8 +577,8 @@ __global__ void __launch_bounds__(kDownWarps * 32, 1) moe_layer_down_kernel(MoeA
         float v[2];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          f2 q = f2_fma(numbers(d2[2 * r], d2[2 * r + 1]), f2_of(256.0f, 256.0f), numbers(d3[2 * r], d3[2 * r + 1]));
-          q = f2_fma(numbers(d1[2 * r], d1[2 * r + 1]), f2_of(65536.0f, 65536.0f), q);
+          f2 q = f2_fma(numbers(d[1][2 * r], d[1][2 * r + 1]), f2_of(256.0f, 256.0f), numbers(d[2][2 * r], d[2][2 * r + 1]));
+          q = f2_fma(numbers(d[0][2 * r], d[0][2 * r + 1]), f2_of(65536.0f, 65536.0f), q);
           q = f2_mul(f2_mul(q, c.s[r]), hs_now);
           if (Raw<QT>::kMin) q = f2_fma(c.m[r], hm_now, q);
           const float2 both = f2_parts(q);
