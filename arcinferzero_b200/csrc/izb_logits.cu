@@ -22,6 +22,7 @@ namespace {
 constexpr int kThreads = 512, kBatch = 5;  // groups of four tokens that a thread has in flight
 constexpr int kRing = (kBatch + 1) * kThreads * 16;
 constexpr int kWords = 16384;              // counting words of a CTA at most (two CTAs per multiprocessor)
+constexpr int kEarly = 8;                  // history tokens that a thread keeps in registers (4096 in all; the rest is read for every window)
 constexpr int kMaxCluster = 16;
 constexpr float kBig = 3.4028234e38f;
 
@@ -93,6 +94,11 @@ __global__ void __launch_bounds__(kThreads, 2) logits_process_kernel(LogitsArgs 
     const int m = p.mask_row ? p.mask_row[r] : r;
     if (m >= 0 && m < p.n_masks) mask = p.mask + (size_t)m * p.mask_words;
   }
+  // (what the first steps wait for is asked for ahead of what fills the queues to memory, and kept for every window)
+  int early[kEarly];
+#pragma unroll
+  for (int j = 0; j < kEarly; ++j) early[j] = h0 + tid + j * kThreads < h1 ? p.hist[h0 + tid + j * kThreads] : -1;
+  const int early_bias = b0 + tid < b1 ? p.bias_ids[b0 + tid] : -1;
   const bool counted = h1 > h0 || b1 > b0, wide = h1 - h0 > 65535 || b1 - b0 > 65535, logz = p.logz != nullptr;
   const int window = p.words ? (wide ? p.words / 2 : p.words) / 4 : groups;  // groups at a time
   uint32_t* s_bias = s_word + 4 * window;                 // (wide: the numbers of the biases)
@@ -130,17 +136,28 @@ __global__ void __launch_bounds__(kThreads, 2) logits_process_kernel(LogitsArgs 
         if (wide) reinterpret_cast<uint4*>(s_bias)[i] = make_uint4(0u, 0u, 0u, 0u);
       }
       __syncthreads();
-      for (int i = b0 + tid; i < b1; i += kThreads) {  // the last entry of a token counts
-        const int v = p.bias_ids[i];
+      auto bias_at = [&](int v, int i) {  // the last entry of a token counts
         const uint32_t at = (uint32_t)v - (uint32_t)first;
         if (v >= 0 && v < p.V && at < (uint32_t)n) atomicMax((wide ? s_bias : s_word) + at, (uint32_t)(i - b0 + 1) << (wide ? 0 : 16));
+      };
+      if (b1 > b0) {
+        bias_at(early_bias, b0 + tid);
+        for (int i = b0 + tid + kThreads; i < b1; i += kThreads) bias_at(p.bias_ids[i], i);
+        __syncthreads();
       }
-      if (b1 > b0) __syncthreads();
-#pragma unroll 4
-      for (int i = h0 + tid; i < h1; i += kThreads) {
-        const int v = p.hist[i];
+      auto count = [&](int v) {
         const uint32_t at = (uint32_t)v - (uint32_t)first;
         if (v >= 0 && v < p.V && at < (uint32_t)n) atomicAdd(s_word + at, 1u);
+      };
+#pragma unroll
+      for (int j = 0; j < kEarly; ++j) count(early[j]);
+#pragma unroll 1
+      for (int i = h0 + tid + kEarly * kThreads; i < h1; i += 4 * kThreads) {
+        int v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = i + j * kThreads < h1 ? p.hist[i + j * kThreads] : -1;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) count(v[j]);
       }
       __syncthreads();
     }
@@ -202,33 +219,38 @@ __global__ void __launch_bounds__(kThreads, 2) logits_process_kernel(LogitsArgs 
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const Top b = {__shfl_xor_sync(0xFFFFFFFFu, top.m, o), __shfl_xor_sync(0xFFFFFFFFu, top.s, o), __shfl_xor_sync(0xFFFFFFFFu, top.at, o)};
-    top = top_join(top, b);
-  }
+  // over the warp, the CTA's warps, the row's CTAs: lane by lane each time
+  auto join = [&](int lanes) {
+#pragma unroll 1
+    for (int o = lanes >> 1; o > 0; o >>= 1) {
+      const Top b = {__shfl_xor_sync(0xFFFFFFFFu, top.m, o), __shfl_xor_sync(0xFFFFFFFFu, top.s, o), __shfl_xor_sync(0xFFFFFFFFu, top.at, o)};
+      top = top_join(top, b);
+    }
+  };
+  join(32);
   if (lane == 0) s_top[warp] = top;
   __syncthreads();
   if (p.cluster > 1) asm volatile("barrier.cluster.wait;" ::: "memory");  // every CTA of the row has begun
-  if (tid == 0) {
-    for (int w = 1; w < kThreads / 32; ++w) top = top_join(top, s_top[w]);
-    if (p.cluster > 1) {  // into the first CTA's shared memory
+  if (warp == 0) {
+    top = s_top[lane & (kThreads / 32 - 1)];
+    join(kThreads / 32);
+    if (p.cluster > 1 && lane == 0) {  // into the first CTA's shared memory
       uint32_t to;
       asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(to) : "r"((uint32_t)__cvta_generic_to_shared(&s_cta[rank])));
       asm volatile("st.shared::cluster.f32 [%0], %1;\n\tst.shared::cluster.f32 [%0+4], %2;\n\tst.shared::cluster.s32 [%0+8], %3;" ::"r"(to), "f"(top.m), "f"(top.s), "r"(top.at)
                    : "memory");
     }
   }
-  if (p.cluster > 1) {
-    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
-    if (rank == 0 && tid == 0) {
-      top = s_cta[0];
-      for (int c = 1; c < p.cluster; ++c) top = top_join(top, s_cta[c]);
+  if (p.cluster > 1) asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+  if (rank == 0 && warp == 0) {
+    if (p.cluster > 1) {
+      top = s_cta[lane & (p.cluster - 1)];  // (a power of two)
+      join(p.cluster);
     }
-  }
-  if (rank == 0 && tid == 0) {
-    if (p.best) p.best[r] = top.at == 0x7FFFFFFF ? 0 : top.at;
-    if (logz) p.logz[r] = logf(top.s) + top.m;
+    if (lane == 0) {
+      if (p.best) p.best[r] = top.at == 0x7FFFFFFF ? 0 : top.at;
+      if (logz) p.logz[r] = logf(top.s) + top.m;
+    }
   }
 }
 
