@@ -19,9 +19,9 @@
 
 namespace {
 
-constexpr int kThreads = 512, kBatch = 5;  // groups of four tokens that a thread has in flight
+constexpr int kThreads = 512, kBatch = 3;  // groups of four tokens that a thread has in flight
 constexpr int kRing = (kBatch + 1) * kThreads * 16;
-constexpr int kWords = 16384;              // counting words of a CTA at most (two CTAs per multiprocessor)
+constexpr int kWords = 19456;              // counting words of a CTA at most (two CTAs per multiprocessor)
 constexpr int kEarly = 8;                  // history tokens that a thread keeps in registers (4096 in all; the rest is read for every window)
 constexpr int kMaxCluster = 16;
 constexpr float kBig = 3.4028234e38f;
