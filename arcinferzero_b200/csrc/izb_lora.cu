@@ -759,8 +759,11 @@ __global__ void __launch_bounds__(kThreads, 2) lora_outer_kernel(LoraArgs p, Row
   if (begin >= end) return;
   const Tile* tiles = reinterpret_cast<const Tile*>(scratch + plan.at_tiles);
 
-  const int col = 4 * (g >> 1) + (g & 1);     // column g of the first instruction; of the second one: two further
-  const int swap = g & 1 ? plan.swap : 0;     // (columns two further are as odd as g)
+  // Column g of the first instruction, and how much further that of the second one is.  Where rows lie on 16-byte boundaries a lane has four neighbouring outputs;
+  // else two and two, so that the four lanes of a row share 32 bytes at a time.
+  const int col = kVec ? 4 * (g >> 1) + (g & 1) : g, col_step = kVec ? 2 : 8, out0 = kVec ? 4 * t : 2 * t;
+  auto out_of = [&](int k) { return kVec ? k : (k >> 1) * 8 + (k & 1); };
+  const int swap = g & 1 ? plan.swap : 0;     // (both columns are as odd as g)
   auto of_u = [&](int k, int group) { return *reinterpret_cast<const uint4*>(smem + ((k * 4 + (warp & 3)) * (ld / 16) + group) * 512 + lane * 16); };
   const int b_row = tid >> 2, b_chunk = tid & 3;  // four threads copy a row of B
   const uint32_t b_to = stages_at + (b_row * ld + (b_chunk ^ (b_row & 1 ? plan.swap : 0)) * 8) * 2, b_swap = b_row & 1 && plan.swap ? 0xFFFFFFC0u : 64u;  // (the next four chunks)
@@ -782,8 +785,8 @@ __global__ void __launch_bounds__(kThreads, 2) lora_outer_kernel(LoraArgs p, Row
     const uint16_t* b_from = p.B + ((size_t)(rank ? tile.adapter : 0) * p.N + step0 * kCols + b_row) * p.R + b_chunk * 8;
     const size_t row = tile.row + m0 + g;
     // (rows past the tile's: the last one again, which nobody stores)
-    const float* from0 = p.base + (size_t)(tile.row + min(m0 + g, tile.rows - 1)) * p.ldb + step0 * kCols + half + 4 * t;
-    const float* from1 = p.base + (size_t)(tile.row + min(m0 + g + 8, tile.rows - 1)) * p.ldb + step0 * kCols + half + 4 * t;
+    const float* from0 = p.base + (size_t)(tile.row + min(m0 + g, tile.rows - 1)) * p.ldb + step0 * kCols + half + out0;
+    const float* from1 = p.base + (size_t)(tile.row + min(m0 + g + 8, tile.rows - 1)) * p.ldb + step0 * kCols + half + out0;
     int ask_n = step0 * kCols;         // the next step's first output
     int ask_left = steps;
     uint32_t ask_at = 0;               // its stage
@@ -811,16 +814,16 @@ __global__ void __launch_bounds__(kThreads, 2) lora_outer_kernel(LoraArgs p, Row
             copy16(to + 2 * kThreads * 16, from0 + 16);
             copy16(to + 3 * kThreads * 16, from1 + 16);
           } else {
-            const int n = ask_n + half + 4 * t;
+            const int n = ask_n + half + out0;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              if (n + k < p.N) {
-                copy4(to + k * 4, from0 + k);
-                copy4(to + kThreads * 16 + k * 4, from1 + k);
+              if (n + out_of(k) < p.N) {
+                copy4(to + k * 4, from0 + out_of(k));
+                copy4(to + kThreads * 16 + k * 4, from1 + out_of(k));
               }
-              if (n + 16 + k < p.N) {
-                copy4(to + 2 * kThreads * 16 + k * 4, from0 + 16 + k);
-                copy4(to + 3 * kThreads * 16 + k * 4, from1 + 16 + k);
+              if (n + 16 + out_of(k) < p.N) {
+                copy4(to + 2 * kThreads * 16 + k * 4, from0 + 16 + out_of(k));
+                copy4(to + 3 * kThreads * 16 + k * 4, from1 + 16 + out_of(k));
               }
             }
           }
@@ -858,8 +861,8 @@ __global__ void __launch_bounds__(kThreads, 2) lora_outer_kernel(LoraArgs p, Row
 
     // ---- outputs
     const unsigned char* here = smem + plan.pieces;
-    float *c0 = p.C + row * p.ldc + step0 * kCols + half + 4 * t, *c1 = c0 + 8 * (size_t)p.ldc;
-    int n = step0 * kCols + half + 4 * t;
+    float *c0 = p.C + row * p.ldc + step0 * kCols + half + out0, *c1 = c0 + 8 * (size_t)p.ldc;
+    int n = step0 * kCols + half + out0;
     for (int i = 0; i < steps; ++i, n += kCols, c0 += kCols, c1 += kCols) {
       copies_there(plan.stages2 - 2);
       __syncthreads();  // this stage has arrived for everybody, and everybody has done with the one before
@@ -871,7 +874,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_outer_kernel(LoraArgs p, Row
       if (m0 >= tile.rows) continue;
       float d[2][2][4] = {};
       // chunks of 32 ranks of B's rows: sixteen outputs h, instruction q
-      auto of_b = [&](int h, int q, int chunk) { return b + (16 * h + 2 * q) * ld + (chunk ^ swap) * 8; };
+      auto of_b = [&](int h, int q, int chunk) { return b + (16 * h + col_step * q) * ld + (chunk ^ swap) * 8; };
       if (kRegs) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -913,7 +916,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_outer_kernel(LoraArgs p, Row
           for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
-              const uint2 v = *reinterpret_cast<const uint2*>(b + (16 * h + 2 * q) * ld + at);
+              const uint2 v = *reinterpret_cast<const uint2*>(b + (16 * h + col_step * q) * ld + at);
               mma<kBf16>(d[h][q], r.x, r.y, r.z, r.w, v.x, v.y);
             }
         }
@@ -929,16 +932,16 @@ __global__ void __launch_bounds__(kThreads, 2) lora_outer_kernel(LoraArgs p, Row
           o0 = make_float4(fmaf(f0, d[h][0][0], o0.x), fmaf(f0, d[h][0][1], o0.y), fmaf(f0, d[h][1][0], o0.z), fmaf(f0, d[h][1][1], o0.w));
           o1 = make_float4(fmaf(f1, d[h][0][2], o1.x), fmaf(f1, d[h][0][3], o1.y), fmaf(f1, d[h][1][2], o1.z), fmaf(f1, d[h][1][3], o1.w));
         }
-        if (kVec && n - half - 4 * t + kCols <= p.N) {
+        if (kVec && n - half - out0 + kCols <= p.N) {
           if (has0) *reinterpret_cast<float4*>(c0 + 16 * h) = o0;
           if (has1) *reinterpret_cast<float4*>(c1 + 16 * h) = o1;
         } else {
           const float v0[4] = {o0.x, o0.y, o0.z, o0.w}, v1[4] = {o1.x, o1.y, o1.z, o1.w};
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            if (n + 16 * h + k < p.N) {
-              if (has0) c0[16 * h + k] = v0[k];
-              if (has1) c1[16 * h + k] = v1[k];
+            if (n + 16 * h + out_of(k) < p.N) {
+              if (has0) c0[16 * h + out_of(k)] = v0[k];
+              if (has1) c1[16 * h + out_of(k)] = v1[k];
             }
         }
       }
