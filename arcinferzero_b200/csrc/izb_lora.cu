@@ -967,7 +967,7 @@ extern "C" int izb_lora_add(int dtype, const void* d_A, const void* d_B, int n_a
   if (!d_A || !d_B || !d_scales || !d_aq || !d_asc || !d_seg || !d_adapter || !d_C) IZB_FAIL(IZB_ERR_ARG, "lora_add: null pointer");
   if (dtype != IZB_F16 && dtype != IZB_BF16) IZB_FAIL(IZB_ERR_TYPE, "lora_add: adapters of type %d are not taken (IZB_F16, IZB_BF16)", dtype);
   if (n_adapters < 1 || R < 16 || R > kMaxRank || R % 16) IZB_FAIL(IZB_ERR_SHAPE, "lora_add: %d adapters of rank %d (16..%d, a multiple of 16: pad with zeros)", n_adapters, R, kMaxRank);
-  if (N < 1 || K < 256 || K % 256) IZB_FAIL(IZB_ERR_SHAPE, "lora_add: N=%d K=%d (K a multiple of 256)", N, K);
+  if (N < 1 || N > 1 << 28 || K < 256 || K > 1 << 28 || K % 256) IZB_FAIL(IZB_ERR_SHAPE, "lora_add: N=%d K=%d (K a multiple of 256, both 2^28 at most)", N, K);
   if (T < 1 || Mp % 16 || Mp < T || n_seg < 1) IZB_FAIL(IZB_ERR_SHAPE, "lora_add: T=%d Mp=%d n_seg=%d (Mp a multiple of 16, >= T)", T, Mp, n_seg);
   if (c_off < 0 || (T > 1 && (int64_t)ldc < (int64_t)c_off + N) || (d_base && T > 1 && ldb < N)) IZB_FAIL(IZB_ERR_SHAPE, "lora_add: N=%d c_off=%d ldc=%d ldb=%d", N, c_off, ldc, ldb);
   if (!izb_aligned(d_A, 16) || !izb_aligned(d_B, 16) || !izb_aligned(d_aq, 16) || !izb_aligned(d_asc, 16))

@@ -249,8 +249,8 @@ int izb_gemm(const izb_weight* w, int mat, const int8_t* d_aq, const float* d_as
  * to it.  d_seg [n_seg + 1]: row offsets, increasing (equal ones: an empty segment); what lies outside 0..T is cut off.  Rows before d_seg[0]
  * and behind the last segment are left as they were.  base: d_base [T][ldb] (its first column), d_base = d_C + c_off with ldb = ldc to add in place, or
  * NULL for zeros; rows of segments without an adapter receive the base.  Sums in f32 in an order that depends on the row's place in its segment's
- * tiles and the call's number of rows and segments alone, not on other rows' values.  A row whose inner sums are no finite numbers is NaN.
- * A, B, aq, asc 16-byte aligned, base and C any f32 address (16-byte aligned rows are faster).  d_scratch: izb_lora_scratch(dtype, R, T, n_seg) bytes (0 for
+ * tiles and the call's number of rows and segments alone, not on other rows' values.  A row whose inner sums are not all finite has no finite
+ * outputs.  A, B, aq, asc 16-byte aligned, base and C any f32 address (16-byte aligned rows are faster).  d_scratch: izb_lora_scratch(dtype, R, T, n_seg) bytes (0 for
  * up to 8 rows per segment on average: then NULL will do), 16-byte aligned, the call's own until it has finished. */
 size_t izb_lora_scratch(int dtype, int R, int T, int n_seg);
 int izb_lora_add(int dtype, const void* d_A, const void* d_B, int n_adapters, int R, const int32_t* d_ranks, const float* d_scales, int N, int K,

@@ -71,6 +71,11 @@ CASES = [
     ([40, 40, 40], [2, 2, 2], [16, 16, 32], 1, 256, "f16"),                      # one output column
     ([129, 31], [0, 1], [80, 112], 15, 1024, "bf16"),
     ([2000, 48], [0, 1], [32, 96], 640, 17408, "f16"),                           # a long K
+    ([3, 2], [1, 0], [128, 112], 100, 512, "f16"),                               # few segments of a few rows: the widest clusters
+    ([8, 7], [0, 1], [256, 16], 64, 768, "bf16"),
+    ([1, 1], [0, 1], [256, 128], 333, 1280, "f16"),                              # single rows of high rank
+    ([1, 1, 1], [0, 1, 0], [48, 80], 70, 512, "bf16"),
+    ([4] * 9, [0, 1, 2] * 3, [16, 32, 64], 200, 512, "f16"),
 ]
 
 
