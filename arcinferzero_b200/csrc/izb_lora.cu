@@ -981,8 +981,11 @@ extern "C" int izb_lora_add(int dtype, const void* d_A, const void* d_B, int n_a
   const bool bf16 = dtype == IZB_BF16, few = few_rows(T, n_seg), one = T <= n_seg;
   const int64_t tiles = (int64_t)T / (one ? 1 : few ? kFewRows : kRows) + n_seg;  // (at most)
   const int sms = izb_sm_count(device);
-  // CTAs per tile.  Few rows: 16 while that leaves the multiprocessors two CTAs at most, else 8.  More rows: as many as fit at once, 8 at most.
-  p.cluster = few && n_seg * 16 <= 2 * sms && R <= 128 ? 16 : 8;
+  // CTAs per tile.  Single rows: as many as leave all of them room at once (64 requests of 17408 x 5120, 4 / 5 / 6 / 8 CTAs: 34.7 / 31.8 / 29.0 / 32.5 us), 4 at
+  // least and 16 at most.  Few rows: 16 while that leaves the multiprocessors two CTAs at most, else 8.  More rows: as many as fit at once, 8 at most.
+  const int widest = R <= 128 ? 16 : 8;
+  if (one) p.cluster = kFewBlocks<1> * sms / T > widest ? widest : kFewBlocks<1> * sms / T < 4 ? 4 : kFewBlocks<1> * sms / T;
+  else p.cluster = few && n_seg * 16ll <= 2 * sms ? widest : 8;
   while (!few && p.cluster > 1 && tiles * p.cluster > 2 * sms) p.cluster /= 2;
   if (tiles * p.cluster > 0x7FFFFFFF) IZB_FAIL(IZB_ERR_LIMIT, "lora_add: %d rows in %d segments", T, n_seg);
   const dim3 grid((unsigned)(tiles * p.cluster));
