@@ -7,12 +7,17 @@
 //   mask bit 0:     l = -inf
 //   temperature>0:  l = l / temperature
 //
-// Every logit is read once and written once: bound by those bytes.  A row is split over a cluster of CTAs, each with a stretch of the vocabulary, so
+// Every logit is read once and written once: bound by those bytes, and with rules on by instruction issue (256 rows of 128256: 48 to 54 us without rules for
+// 40 us of bytes, 85 with all of them at 70 % of the issue slots).  A row is split over a cluster of CTAs, each with a stretch of the vocabulary, so
 // that a single row has 16 multiprocessors at work; what is joined at the end is one (maximum, index, sum) per CTA, through distributed shared memory,
-// in the order of the stretches.  A CTA first asks for its logits (five 16-byte loads per thread in flight), then counts: one word of shared
-// memory per token of the stretch, the count of the history in its lower half and the number of the bias in the upper one.  Every CTA of a row reads
-// the row's whole history, since most of it belongs to others: handing tokens on through distributed shared memory would save less than
-// the cluster-wide barrier costs.  Rows with more than 65535 of either take two words per token and half the stretch at a time.
+// in the order of the stretches.  A CTA first asks for the row's history, then for its logits (three 16-byte copies per thread in flight, into a ring; loads
+// into as many registers share scoreboards and wait for one another, 84 against 67 us), then counts: one word of shared memory per token of a window of the
+// stretch, the count of the history in its lower half and the number of the bias in the upper one.  Every CTA of a row reads the row's whole history, since
+// most of it belongs to others: handing tokens on through distributed shared memory would save less than the cluster-wide barrier costs.  Rows with more than
+// 65535 of either take two words per token and half the window at a time.
+// (Taken back: a bitmap of the tokens that the rules touch, and counts for those alone, numbered by its running sum.  The pass over the others is then
+// free of rules, but the steps before it wait for memory one after the other: 64 rows 55 us against 36.  The touched tokens of a lane one by one instead of its
+// four together: 93 against 85 for 256 rows, by the registers it takes.)
 #include <math.h>
 
 #include "izb_common.cuh"
@@ -263,6 +268,7 @@ extern "C" int izb_logits_process(const float* d_logits, int ldl, float* d_out, 
   if (rows < 1 || V < 1 || V > 1 << 30 || (rows > 1 && (ldl < V || ldo < V))) IZB_FAIL(IZB_ERR_SHAPE, "logits_process: rows=%d V=%d ldl=%d ldo=%d (ldl, ldo >= V)", rows, V, ldl, ldo);
   if (n_hist < 0 || (n_hist && (!d_hist || !d_hist_off)) || n_bias < 0 || (n_bias && (!d_bias_ids || !d_bias || !d_bias_off)))
     IZB_FAIL(IZB_ERR_ARG, "logits_process: %d history tokens, %d biases and a null pointer among their arrays", n_hist, n_bias);
+  if (n_hist > 1 << 30 || n_bias > 1 << 30) IZB_FAIL(IZB_ERR_LIMIT, "logits_process: %d history tokens, %d biases (2^30 at most)", n_hist, n_bias);
   if (n_hist && !d_params) IZB_FAIL(IZB_ERR_ARG, "logits_process: a history without the penalties' parameters");
   if (d_mask && (mask_words < 0 || (int64_t)mask_words * 32 < V || n_masks < 1 || (!d_mask_row && n_masks < rows)))
     IZB_FAIL(IZB_ERR_SHAPE, "logits_process: %d masks of %d words for %d rows of %d tokens", n_masks, mask_words, rows, V);
@@ -276,8 +282,8 @@ extern "C" int izb_logits_process(const float* d_logits, int ldl, float* d_out, 
   p.mask = d_mask; p.mask_row = d_mask_row;
   p.best = d_best; p.logz = d_logz;
   p.ldl = ldl; p.ldo = ldo; p.V = V; p.n_hist = n_hist; p.n_bias = n_bias; p.mask_words = mask_words; p.n_masks = n_masks;
-  // How many CTAs share a row: 16 while that leaves the multiprocessors two CTAs at most (one row of 151936: see above), else 4 (64 rows of 151936, CTAs
-  // per row 1 / 2 / 4 / 8: 108 / 67 / 41 / 46 us; 256 rows of 128256: 94 / 85 / 86 / 100), and no more than give every thread a group.
+  // How many CTAs share a row: 16 while that leaves the multiprocessors two CTAs at most, else 4 (64 rows of 151936, CTAs per row 2 / 4 / 8: 63 / 38 / 44 us;
+  // 256 rows of 128256: 86 / 86 / 102; without rules 24 / 16 / 21 and 50 / 54 / 69), and no more than give every thread a group.
   int device = 0;
   IZB_CUDA(cudaGetDevice(&device));
   const int groups = V / 4 + 2;

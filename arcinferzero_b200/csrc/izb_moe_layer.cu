@@ -6,16 +6,23 @@
 //
 // Bound by the bytes of the experts that the tokens reach, each read once.  Both kernels work on 16 weight rows x one superblock per warp (lane
 // g = lane / 4, t = lane % 4 holds bytes 8t .. 8t+7 of each block of rows g and g + 8).  A warp has a ring of such pieces of its own in shared memory,
-// filled by 16-byte asynchronous copies, and asks for the next piece as soon as it has one in registers, across the borders of experts and channels:
-// 110 to 150 KB per multiprocessor are on their way all the time.
+// filled by 16-byte asynchronous copies, and asks for the next piece as soon as it has one in registers, across the borders of experts and channels.
 // Most experts have one or two tokens, for which an instruction with a token per column is mostly empty and a lane repeats a row's scales for all of
 // its blocks.  So the columns are the eight blocks of the superblock instead: the B operand of block b's instruction has the token's values in
 // column b and zeros beside them, eight instructions add up to the 16 x 8 block sums, and lane t scales blocks 2t and 2t + 1 of its two rows -- each
 // scale is decoded by one lane, once.  What comes after is a sum over the quad.
 //
-// Routing is done by every CTA for itself (a warp per token, a microsecond less than a launch).  The first kernel lets the second one in behind its own
-// wait for the kernel before: what was written before this call is then visible to the second kernel from its start, and it routes and asks for its first
-// weights while the first kernel still runs.
+// Routing is done by every CTA for itself (a warp per token; 2.6 us, with what follows from it, against a launch and its hand-over).  The first kernel lets the
+// second one in behind its own wait for the kernel before: what was written before this call is then visible to the second kernel from its start, and it routes
+// and asks for its first weights while the first kernel still runs.
+//
+// Measured (us; the six calls / this; the floor by bytes), 128 experts of 768 over 2048, top 8, Q4_K: one token 26 / 18 (3.3), four 48 / 36, eight 88 / 55 (21),
+// 16 154 / 88, 32 208 / 147 (45); 60 experts of 1280 over 4096, top 4, five tokens 99 / 56.  Many tokens per expert are where the block-per-column form has nothing
+// to gain (it costs every token eight instructions): 8 experts, top 2, 32 tokens 47 / 55.  One token is latency: routing 2.6 us, first bytes of weights 2.4, the
+// barriers.  Eight tokens: the first kernel's loop runs at 4.1 TB/s, the second one's at 2.9, both near 48 % of the issue slots with 16 warps per multiprocessor:
+// a superblock of gate and up takes about 560 instructions, of which decoding 6-bit scales is a fifth.
+// (Taken back: 24 warps per multiprocessor with gate and up one after the other and 80 registers, 55 -> 82 us; calling the routing and the epilogues once on
+// zeros so that their code is in the cache, 18 -> 23.)
 #include "izb_common.cuh"
 
 namespace {

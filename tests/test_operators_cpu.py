@@ -68,6 +68,15 @@ def test_logits_process_refuses():
         assert logits(**kw) == status, (kw, izb.lib().izb_last_error())
 
 
+def test_logits_process_refuses_arrays_past_its_numbers():
+    """Positions in the arrays are 32-bit numbers that the kernel adds strides to."""
+    q = p(aligned(65536))
+    for n, status in (((1 << 30) + 1, LIMIT), (2 ** 31 - 1, LIMIT)):
+        assert logits(n_hist=n, params=q, hist=q, hist_off=q) == status
+        assert logits(n_bias=n, bias_ids=q, bias=q, bias_off=q) == status
+    assert logits(V=(1 << 30) + 1, ldl=(1 << 30) + 1, ldo=(1 << 30) + 1) == SHAPE
+
+
 def test_moe_layer_refuses_without_weights():
     L = izb.lib()
     q = p(aligned(64))
