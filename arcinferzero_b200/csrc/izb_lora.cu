@@ -711,7 +711,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_inner_kernel(LoraArgs p, Row
   __syncthreads();
   cluster_wait();  // every CTA has begun
   // the CTA's sums, four ranks per thread, to the CTA that joins these rows
-  const int own = kRows / p.cluster;  // (8, 16, 32 or 64)
+  const int own = kRows / p.cluster;  // (4, 8, 16, 32 or 64)
   {
     const int row = tid >> 2;
     for (int j = (tid & 3) * 4; j < rank && row < tile.rows; j += 16) {
@@ -841,16 +841,19 @@ __global__ void __launch_bounds__(kThreads, 2) lora_outer_kernel(LoraArgs p, Row
       }
       copies_begun();
     };
+    // ---- u's pieces, then the first stages
+    if (rank) {
+      const unsigned char* from = scratch + plan.at_pieces + (size_t)index * plan.pieces;
+      for (uint32_t k = tid * 16; k < plan.pieces; k += kThreads * 16) copy16(smem_at + k, from + k);
+      copies_begun();
+    }
     for (int i = 0; i < plan.stages2 - 1; ++i) ask();
-
-    // ---- u's pieces
     float f0 = 0.0f, f1 = 0.0f;
     if (rank) {
-      const uint4* from = reinterpret_cast<const uint4*>(scratch + plan.at_pieces + (size_t)index * plan.pieces);
-      for (uint32_t k = tid; k < plan.pieces / 16; k += kThreads) reinterpret_cast<uint4*>(smem)[k] = from[k];
       const float* factors = reinterpret_cast<const float*>(scratch + plan.at_factors) + (size_t)index * kRows + m0 + g;
       f0 = factors[0];
       f1 = factors[8];
+      copies_there(plan.stages2 - 1);
       __syncthreads();
       if (kRegs) {
 #pragma unroll
@@ -987,11 +990,14 @@ extern "C" int izb_lora_add(int dtype, const void* d_A, const void* d_B, int n_a
   const int64_t tiles = (int64_t)T / (one ? 1 : few ? kFewRows : kRows) + n_seg;  // (at most)
   const int sms = izb_sm_count(device);
   // CTAs per tile.  Single rows: as many as leave all of them room at once (64 requests of 17408 x 5120, 4 / 5 / 6 / 8 CTAs: 34.7 / 31.8 / 29.0 / 32.5 us), 4 at
-  // least and 16 at most.  Few rows: 16 while that leaves the multiprocessors two CTAs at most, else 8.  More rows: as many as fit at once, 8 at most.
+  // least and 16 at most.  Few rows: 16 while that leaves the multiprocessors two CTAs at most, else 8.  More rows: as many as fit at once, 16 at most, where
+  // cuts of segments that are no multiple of 64 rows leave half a tile each (8 at most and a tile each before: 451 rows of 14592, rank 128, 50 us against 33; 2210
+  // rows of 16128 in 46 segments, rank 16, 77 against 51).
   const int widest = R <= 128 ? 16 : 8;
   if (one) p.cluster = kFewBlocks<1> * sms / T > widest ? widest : kFewBlocks<1> * sms / T < 4 ? 4 : kFewBlocks<1> * sms / T;
   else p.cluster = few && n_seg * 16ll <= 2 * sms ? widest : 8;
-  while (!few && p.cluster > 1 && tiles * p.cluster > 2 * sms) p.cluster /= 2;
+  if (!few)
+    for (p.cluster = 16; p.cluster > 1 && (T / kRows + (n_seg + 1ll) / 2) * p.cluster > 2 * sms;) p.cluster /= 2;
   if (tiles * p.cluster > 0x7FFFFFFF) IZB_FAIL(IZB_ERR_LIMIT, "lora_add: %d rows in %d segments", T, n_seg);
   const dim3 grid((unsigned)(tiles * p.cluster));
   if (few) {
@@ -1025,6 +1031,7 @@ extern "C" int izb_lora_add(int dtype, const void* d_A, const void* d_B, int n_a
     return rc;
   if (int rc = once[8 + bf16].run(device, [&]() -> int {
         IZB_CUDA(cudaFuncSetAttribute(inner, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxInner));
+        IZB_CUDA(cudaFuncSetAttribute(inner, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
         return IZB_OK;
       }))
     return rc;
