@@ -578,6 +578,9 @@ __global__ void __launch_bounds__(kThreads, kFewBlocks<kRowsOf>) lora_few_kernel
 // ---------------------------------------------------------------------------------------------- up to 64 rows
 constexpr int kRows = 64;         // rows of a tile
 constexpr int kCols = 64;         // outputs of a step of the second product
+constexpr int kPitch = 72;        // floats of a step's row in shared memory where it starts anywhere (up to 17 chunks of 16 bytes)
+// Where rows of base and outputs start: both on 16-byte boundaries; anywhere, but each row's two alike; anywhere
+enum { kOnLines, kAlike, kAnywhere };
 // A's and B's tiles: rows of whole 64 bytes in 16-byte chunks; where a row is a multiple of 128 bytes odd rows have the halves of their
 // 128-byte lines changed over, so that two neighbouring rows' 64 bytes lie on different banks.
 struct RowsPlan {
@@ -588,7 +591,7 @@ struct RowsPlan {
   uint32_t all, total1;               // first product: the CTAs' sums lie behind the stages and, over them, the warps' sums
   uint32_t pieces, total2;            // second product: u's pieces, then stages
   uint32_t at_tiles, at_factors, at_pieces;  // scratch: number of tiles | Tile each | 64 factors each | pieces each
-  RowsPlan(int R, bool bf16, size_t tiles) {
+  RowsPlan(int R, bool bf16, size_t tiles, int place = kOnLines) {
     groups = R <= 64 ? 1 : R <= 128 ? 2 : 4;
     parts = kWarps / 2 / groups;
     ld = (R + 31) / 32 * 32;
@@ -598,13 +601,14 @@ struct RowsPlan {
     all = part > 3 * stage1 ? part : 3 * stage1;
     total1 = all + (uint32_t)kRows * (R + 8) * 4;
     pieces = (bf16 ? 3 : 2) * kRows * ld * 2;
-    stage2 = kCols * ld * 2 + kRows * kCols * 4;
+    stage2 = kCols * ld * 2 + kRows * (place == kAlike ? kPitch : kCols) * 4;
     stages2 = R <= 128 ? 3 : 2;
     total2 = pieces + stages2 * stage2;
     at_tiles = 16;
     at_factors = (uint32_t)(at_tiles + tiles * sizeof(Tile) + 15) / 16 * 16;
     at_pieces = (uint32_t)(at_factors + tiles * kRows * 4);
   }
+  static constexpr int kMost2 = 204 << 10;   // total2 at most (R = 256, bf16: 98304 + 2 * (32768 + 18432))
   size_t scratch(size_t tiles) const { return at_pieces + tiles * pieces; }
 };
 // The first product: u's pieces, rows' factors and the tile's place, into scratch.
@@ -749,13 +753,18 @@ __global__ void __launch_bounds__(kThreads, 2) lora_inner_kernel(LoraArgs p, Row
 
 // The second product, base and outputs: steps of 64 rows x 64 outputs, an equal stretch of all of them for each CTA.
 // kRegs: the ranks are 64 at most, and a warp holds its rows' pieces in registers
-template <bool kBf16, bool kVec, bool kRegs>
+// kPlace: what base and outputs go through.  On boundaries a lane copies the 16 bytes that it adds to, and stores 16 bytes.  Where each row of the base starts as
+// far from a boundary as the outputs' row, a step's 64 x 64 go through shared memory as they lie in memory, 16-byte chunks from boundary to boundary, both ways;
+// a chunk is copied and stored by one thread, so that no barrier is needed for it to be filled again.  Else single values (6469 rows, 1024 -> 3416, rows of 3419:
+// 126 us, through shared memory 91).
+template <bool kBf16, int kPlace, bool kRegs>
 __global__ void __launch_bounds__(kThreads, 2) lora_outer_kernel(LoraArgs p, RowsPlan plan, const unsigned char* scratch) {
   extern __shared__ __align__(16) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3, ld = plan.ld;
   const int m0 = (warp & 3) * 16, half = (warp >> 2) * 32;  // a warp has 16 rows and 32 of the 64 outputs
   const uint32_t smem_at = (uint32_t)__cvta_generic_to_shared(smem), stages_at = smem_at + plan.pieces;
   const bool in_place = p.base == p.C;
+  constexpr bool kVec = kPlace == kOnLines;
   pdl_launch_next();
   pdl_wait();
   const int per = (p.N + kCols - 1) / kCols;
@@ -772,7 +781,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_outer_kernel(LoraArgs p, Row
   auto of_u = [&](int k, int group) { return *reinterpret_cast<const uint4*>(smem + ((k * 4 + (warp & 3)) * (ld / 16) + group) * 512 + lane * 16); };
   const int b_row = tid >> 2, b_chunk = tid & 3;  // four threads copy a row of B
   const uint32_t b_to = stages_at + (b_row * ld + (b_chunk ^ (b_row & 1 ? plan.swap : 0)) * 8) * 2, b_swap = b_row & 1 && plan.swap ? 0xFFFFFFC0u : 64u;  // (the next four chunks)
-  const uint32_t base_to = stages_at + kCols * ld * 2 + tid * 16;
+  const uint32_t base_to = stages_at + kCols * ld * 2 + (kPlace == kAlike ? (b_row * kPitch + b_chunk * 4) * 4 : tid * 16);
   uint4 held[kRegs ? 2 : 1][kPieces<kBf16>][2] = {};
 
   // A tile's steps in this CTA's stretch, one tile after the other
@@ -792,6 +801,29 @@ __global__ void __launch_bounds__(kThreads, 2) lora_outer_kernel(LoraArgs p, Row
     // (rows past the tile's: the last one again, which nobody stores)
     const float* from0 = p.base + (size_t)(tile.row + min(m0 + g, tile.rows - 1)) * p.ldb + step0 * kCols + half + out0;
     const float* from1 = p.base + (size_t)(tile.row + min(m0 + g + 8, tile.rows - 1)) * p.ldb + step0 * kCols + half + out0;
+    // (kAlike: what this thread copies and stores, of row b_row the chunks b_chunk, b_chunk + 4, ...; chunk c holds the step's outputs 4c - shift .. 4c - shift + 3)
+    const float* line_from = p.base + (size_t)(tile.row + min(b_row, tile.rows - 1)) * p.ldb;
+    float* line_to = p.C + (size_t)(tile.row + min(b_row, tile.rows - 1)) * p.ldc;
+    auto shift_of = [&](const float* at) { return (int)((uintptr_t)at >> 2) & 3; };
+    const int shift = shift_of(line_to), chunks = b_row < tile.rows ? (kCols + shift + 3) / 4 : 0;
+    auto store = [&](const unsigned char* stage, int n) {  // the step from output n on
+      const float* from = reinterpret_cast<const float*>(stage + kCols * ld * 2) + b_row * kPitch;
+#pragma unroll
+      for (int j = 0; j < 5; ++j) {
+        const int c = b_chunk + 4 * j, lo = 4 * c - shift;
+        if (c >= chunks) break;
+        const float4 v = *reinterpret_cast<const float4*>(from + 4 * c);
+        float* to = line_to + n + lo;
+        if (lo >= 0 && lo + 4 <= kCols && n + lo + 4 <= p.N) {
+          *reinterpret_cast<float4*>(to) = v;
+        } else {
+          const float w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (lo + k >= 0 && lo + k < kCols && n + lo + k < p.N) to[k] = w[k];
+        }
+      }
+    };
     int ask_n = step0 * kCols;         // the next step's first output
     int ask_left = steps;
     uint32_t ask_at = 0;               // its stage
@@ -813,7 +845,20 @@ __global__ void __launch_bounds__(kThreads, 2) lora_outer_kernel(LoraArgs p, Row
         b_from += (size_t)kCols * p.R;
         if (p.base) {
           const uint32_t to = base_to + ask_at;
-          if (kVec && ask_n + kCols <= p.N) {
+          if (kPlace == kAlike) {
+#pragma unroll
+            for (int j = 0; j < 5; ++j) {
+              const int c = b_chunk + 4 * j, n = ask_n + 4 * c - shift;
+              if (c >= chunks) break;
+              if (n >= 0 && n + 4 <= p.N) {
+                copy16(to + j * 64, line_from + n);
+              } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                  if (n + k >= 0 && n + k < p.N) copy4(to + j * 64 + k * 4, line_from + n + k);
+              }
+            }
+          } else if (kVec && ask_n + kCols <= p.N) {
             copy16(to, from0);
             copy16(to + kThreads * 16, from1);
             copy16(to + 2 * kThreads * 16, from0 + 16);
@@ -868,12 +913,20 @@ __global__ void __launch_bounds__(kThreads, 2) lora_outer_kernel(LoraArgs p, Row
     }
 
     // ---- outputs
-    const unsigned char* here = smem + plan.pieces;
+    const unsigned char *here = smem + plan.pieces, *stage = here;
+    int at0 = 0, at1 = 0;  // (kAlike: where this lane's first outputs of rows g and g + 8 are in a stage)
+    if (kPlace == kAlike) {
+      const int r0 = m0 + g, r1 = m0 + g + 8;
+      at0 = r0 * kPitch + half + out0 + shift_of(p.C + (size_t)(tile.row + r0) * p.ldc);
+      at1 = r1 * kPitch + half + out0 + shift_of(p.C + (size_t)(tile.row + r1) * p.ldc);
+    }
     float *c0 = p.C + row * p.ldc + step0 * kCols + half + out0, *c1 = c0 + 8 * (size_t)p.ldc;
     int n = step0 * kCols + half + out0;
     for (int i = 0; i < steps; ++i, n += kCols, c0 += kCols, c1 += kCols) {
       copies_there(plan.stages2 - 2);
       __syncthreads();  // this stage has arrived for everybody, and everybody has done with the one before
+      if (kPlace == kAlike && i) store(stage, n - kCols - half - out0);
+      stage = here;
       ask();
       const uint16_t* b = reinterpret_cast<const uint16_t*>(here) + (half + col) * ld + t * 8;
       const float4* old = reinterpret_cast<const float4*>(here + kCols * ld * 2) + tid;
@@ -932,7 +985,16 @@ __global__ void __launch_bounds__(kThreads, 2) lora_outer_kernel(LoraArgs p, Row
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float4 o0 = make_float4(0.0f, 0.0f, 0.0f, 0.0f), o1 = o0;
-        if (p.base) {
+        float *s0 = nullptr, *s1 = nullptr;
+        if (kPlace == kAlike) {
+          float* line = const_cast<float*>(reinterpret_cast<const float*>(stage + kCols * ld * 2)) + 16 * h;
+          s0 = line + at0;
+          s1 = line + at1;
+          if (p.base) {
+            o0 = make_float4(s0[out_of(0)], s0[out_of(1)], s0[out_of(2)], s0[out_of(3)]);
+            o1 = make_float4(s1[out_of(0)], s1[out_of(1)], s1[out_of(2)], s1[out_of(3)]);
+          }
+        } else if (p.base) {
           o0 = old[2 * h * kThreads];
           o1 = old[(2 * h + 1) * kThreads];
         }
@@ -940,7 +1002,14 @@ __global__ void __launch_bounds__(kThreads, 2) lora_outer_kernel(LoraArgs p, Row
           o0 = make_float4(fmaf(f0, d[h][0][0], o0.x), fmaf(f0, d[h][0][1], o0.y), fmaf(f0, d[h][1][0], o0.z), fmaf(f0, d[h][1][1], o0.w));
           o1 = make_float4(fmaf(f1, d[h][0][2], o1.x), fmaf(f1, d[h][0][3], o1.y), fmaf(f1, d[h][1][2], o1.z), fmaf(f1, d[h][1][3], o1.w));
         }
-        if (kVec && n - half - out0 + kCols <= p.N) {
+        if (kPlace == kAlike) {
+          const float v0[4] = {o0.x, o0.y, o0.z, o0.w}, v1[4] = {o1.x, o1.y, o1.z, o1.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            s0[out_of(k)] = v0[k];
+            s1[out_of(k)] = v1[k];
+          }
+        } else if (kVec && n - half - out0 + kCols <= p.N) {
           if (has0) *reinterpret_cast<float4*>(c0 + 16 * h) = o0;
           if (has1) *reinterpret_cast<float4*>(c1 + 16 * h) = o1;
         } else {
@@ -955,6 +1024,10 @@ __global__ void __launch_bounds__(kThreads, 2) lora_outer_kernel(LoraArgs p, Row
       }
     }
     copies_there<0>();
+    if (kPlace == kAlike) {
+      __syncthreads();
+      store(stage, n - kCols - half - out0);
+    }
   }
 }
 
@@ -1015,21 +1088,23 @@ extern "C" int izb_lora_add(int dtype, const void* d_A, const void* d_B, int n_a
     return IZB_OK;
   }
   if (!d_scratch || !izb_aligned(d_scratch, 16)) IZB_FAIL(IZB_ERR_ARG, "lora_add: %d rows in %d segments want %zu bytes of scratch, 16-byte aligned", T, n_seg, izb_lora_scratch(dtype, R, T, n_seg));
-  const RowsPlan plan(R, bf16, tiles);
-  if (plan.scratch(tiles) > 0xFFFFFFFFu) IZB_FAIL(IZB_ERR_LIMIT, "lora_add: %d rows in %d segments of rank %d", T, n_seg, R);
+  if (RowsPlan(R, bf16, tiles).scratch(tiles) > 0xFFFFFFFFu) IZB_FAIL(IZB_ERR_LIMIT, "lora_add: %d rows in %d segments of rank %d", T, n_seg, R);
   const bool vec = izb_aligned(p.C, 16) && ldc % 4 == 0 && (!d_base || (izb_aligned(d_base, 16) && ldb % 4 == 0));
-  static izb_device_once once[10];
+  const int place = vec ? kOnLines : !d_base || (((uintptr_t)p.C - (uintptr_t)d_base) % 16 == 0 && (ldc - (int64_t)ldb) % 4 == 0) ? kAlike : kAnywhere;
+  const RowsPlan plan(R, bf16, tiles, place);
+  static izb_device_once once[14];
   void (*const inner)(LoraArgs, RowsPlan, unsigned char*) = bf16 ? lora_inner_kernel<true> : lora_inner_kernel<false>;
-  void (*const outers[8])(LoraArgs, RowsPlan, const unsigned char*) = {lora_outer_kernel<false, false, false>, lora_outer_kernel<false, false, true>, lora_outer_kernel<false, true, false>,
-                                                                       lora_outer_kernel<false, true, true>, lora_outer_kernel<true, false, false>, lora_outer_kernel<true, false, true>,
-                                                                       lora_outer_kernel<true, true, false>, lora_outer_kernel<true, true, true>};
-  const int which = (bf16 ? 4 : 0) + (vec ? 2 : 0) + (R <= 64 ? 1 : 0);
+  void (*const outers[12])(LoraArgs, RowsPlan, const unsigned char*) = {
+      lora_outer_kernel<false, kOnLines, false>, lora_outer_kernel<false, kOnLines, true>, lora_outer_kernel<false, kAlike, false>, lora_outer_kernel<false, kAlike, true>,
+      lora_outer_kernel<false, kAnywhere, false>, lora_outer_kernel<false, kAnywhere, true>, lora_outer_kernel<true, kOnLines, false>, lora_outer_kernel<true, kOnLines, true>,
+      lora_outer_kernel<true, kAlike, false>, lora_outer_kernel<true, kAlike, true>, lora_outer_kernel<true, kAnywhere, false>, lora_outer_kernel<true, kAnywhere, true>};
+  const int which = (bf16 ? 6 : 0) + 2 * place + (R <= 64 ? 1 : 0);
   if (int rc = once[which].run(device, [&]() -> int {
-        IZB_CUDA(cudaFuncSetAttribute(outers[which], cudaFuncAttributeMaxDynamicSharedMemorySize, (int)RowsPlan(R <= 64 ? 64 : kMaxRank, true, 0).total2));
+        IZB_CUDA(cudaFuncSetAttribute(outers[which], cudaFuncAttributeMaxDynamicSharedMemorySize, RowsPlan::kMost2));
         return IZB_OK;
       }))
     return rc;
-  if (int rc = once[8 + bf16].run(device, [&]() -> int {
+  if (int rc = once[12 + bf16].run(device, [&]() -> int {
         IZB_CUDA(cudaFuncSetAttribute(inner, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxInner));
         IZB_CUDA(cudaFuncSetAttribute(inner, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
         return IZB_OK;

@@ -201,3 +201,37 @@ def test_refused_by_the_binding(izb, torch):
             bad(**kw)
     with pytest.raises(izb.IzbError):
         bad(A=c.A[:, :8].contiguous(), B=c.B[:, :, :8].contiguous())
+
+
+@pytest.mark.parametrize("lens,adapters,ranks,N,K,dtype", [
+    ([70, 1, 33, 64, 65, 128], [0, 1, 2, -1, 0, 2], [64, 16, 48], 777, 512, "bf16"),
+    ([700, 90], [0, 1], [32, 80], 1001, 256, "f16"),
+    ([640], [0], [256], 1499, 256, "bf16"),
+    ([64, 9, 130], [0, 0, 0], [16], 67, 256, "f16"),
+    ([20], [0], [128], 3, 256, "f16")])
+def test_prompts_rows_wherever_they_start(izb, torch, lens, adapters, ranks, N, K, dtype):
+    """Base and outputs in windows of wider buffers: the bits are those of rows on 16-byte boundaries, and what is beside the windows stays."""
+    c = Case(izb, torch, lens, adapters, ranks, N, K, dtype, first=1, behind=3)
+    T, last = c.T, c.first + sum(lens)
+    lines = torch.empty((T, (N + 3) // 4 * 4), device="cuda")[:, :N]
+    on = torch.zeros((T, (N + 3) // 4 * 4), device="cuda")[:, :N]
+    lines.copy_(c.base)
+    izb.lora_add(*c.args(), on, base=lines, ranks=c.rk)
+    want, room = c.want(c.base)
+    assert off(on[c.first:last], want[c.first:last], room[c.first:last]) <= 1
+    #            columns before and behind, of the outputs and of the base (None: in place)
+    for c0, c1, b0, b1 in ((0, 1, None, 0), (1, 2, None, 0), (3, 0, None, 0), (2, 5, None, 0), (1, 4, 5, 4), (2, 3, 2, 3), (3, 3, 7, 3), (1, 1, 0, 2), (0, 3, 1, 1)):
+        wide = torch.full((T, c0 + N + c1), 7.0, device="cuda")
+        if b0 is None:
+            wide[:, c0:c0 + N] = c.base
+            izb.lora_add(*c.args(), wide, c_off=c0, ranks=c.rk)
+            rest = c.base
+        else:
+            base = torch.full((T, b0 + N + b1), float("nan"), device="cuda")
+            base[:, b0:b0 + N] = c.base
+            izb.lora_add(*c.args(), wide, base=base[:, b0:b0 + N], c_off=c0, ranks=c.rk)
+            rest = torch.full((T, N), 7.0, device="cuda")
+        got = wide[:, c0:c0 + N]
+        assert torch.equal(got[c.first:last], on[c.first:last]), (c0, c1, b0, b1)
+        assert torch.equal(got[:c.first], rest[:c.first]) and torch.equal(got[last:], rest[last:])
+        assert bool((wide[:, :c0] == 7.0).all() and (wide[:, c0 + N:] == 7.0).all())
