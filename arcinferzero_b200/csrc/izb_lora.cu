@@ -602,13 +602,15 @@ struct RowsPlan {
     total1 = all + (uint32_t)kRows * (R + 8) * 4;
     pieces = (bf16 ? 3 : 2) * kRows * ld * 2;
     stage2 = kCols * ld * 2 + kRows * (place == kAlike ? kPitch : kCols) * 4;
-    stages2 = R <= 128 ? 3 : 2;
+    const uint32_t half_sm = (228 << 10) / 2 - 1024;
+    auto fits = [&](int stages, uint32_t room) { return pieces + stages * stage2 <= room; };
+    stages2 = fits(3, half_sm) || (!fits(2, half_sm) && fits(3, kMost2)) ? 3 : 2;  // (two CTAs per multiprocessor before a third stage)
     total2 = pieces + stages2 * stage2;
     at_tiles = 16;
     at_factors = (uint32_t)(at_tiles + tiles * sizeof(Tile) + 15) / 16 * 16;
     at_pieces = (uint32_t)(at_factors + tiles * kRows * 4);
   }
-  static constexpr int kMost2 = 204 << 10;   // total2 at most (R = 256, bf16: 98304 + 2 * (32768 + 18432))
+  static constexpr int kMost2 = 227 << 10;   // total2 at most
   size_t scratch(size_t tiles) const { return at_pieces + tiles * pieces; }
 };
 // The first product: u's pieces, rows' factors and the tile's place, into scratch.
@@ -756,7 +758,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_inner_kernel(LoraArgs p, Row
 // kPlace: what base and outputs go through.  On boundaries a lane copies the 16 bytes that it adds to, and stores 16 bytes.  Where each row of the base starts as
 // far from a boundary as the outputs' row, a step's 64 x 64 go through shared memory as they lie in memory, 16-byte chunks from boundary to boundary, both ways;
 // a chunk is copied and stored by one thread, so that no barrier is needed for it to be filled again.  Else single values (6469 rows, 1024 -> 3416, rows of 3419:
-// 126 us, through shared memory 91).
+// 126 us, through shared memory 104).
 template <bool kBf16, int kPlace, bool kRegs>
 __global__ void __launch_bounds__(kThreads, 2) lora_outer_kernel(LoraArgs p, RowsPlan plan, const unsigned char* scratch) {
   extern __shared__ __align__(16) unsigned char smem[];
@@ -889,7 +891,13 @@ __global__ void __launch_bounds__(kThreads, 2) lora_outer_kernel(LoraArgs p, Row
     // ---- u's pieces, then the first stages
     if (rank) {
       const unsigned char* from = scratch + plan.at_pieces + (size_t)index * plan.pieces;
-      for (uint32_t k = tid * 16; k < plan.pieces; k += kThreads * 16) copy16(smem_at + k, from + k);
+      // (of each piece's sixteen rows what the rank fills)
+      if (kRegs || rank + 16 > ld) {
+        for (uint32_t k = tid * 16; k < plan.pieces; k += kThreads * 16) copy16(smem_at + k, from + k);
+      } else {
+        for (uint32_t k = tid * 16; k < plan.pieces; k += kThreads * 16)
+          if (k % (ld * 32u) < rank * 32u) copy16(smem_at + k, from + k);
+      }
       copies_begun();
     }
     for (int i = 0; i < plan.stages2 - 1; ++i) ask();
