@@ -40,7 +40,7 @@ struct MoeArgs {
   int8_t* hq;         // [T * NU][3][F]
   float *hs, *hsum;   // [T * NU][F / 32]: the power of two, the sum of the block's values
   float* out;
-  int T, Mp, ldl, NE, NU, e0, n_mats, E, F, joined, splits;
+  int T, Mp, ldl, NE, NU, e0, n_mats, E, F, joined, splits, cluster;
   size_t gate_row, down_row;  // bytes of a row
 };
 
@@ -467,7 +467,9 @@ __global__ void __launch_bounds__(kUpWarps * 32, 2) moe_layer_up_kernel(MoeArgs 
 
 // ---------------------------------------------------------------------------------------------- down, combine
 // A CTA takes 16 outputs of all tokens; its warps the experts, each in `splits` parts of F (by F alone, so that a token's sums do not depend on
-// which others the call has).
+// which others the call has).  Where there are few outputs a cluster of CTAs takes 16 of them, each its share of the experts: their sums go to the first
+// one's shared memory, the last step of each straight from registers (us
+// without / with: 25 tokens, 512 outputs, F 768, 6 experts, top 5 59 / 46; 31 tokens, 768 outputs, F 512, 19 experts, top 6 53 / 45).
 template <int QT>
 struct Down {
   static constexpr int kSlots = QT == IZB_Q4_K ? 3 : 2, kSlot = Copier<QT>::kTile;
@@ -490,7 +492,7 @@ __device__ __forceinline__ void down_combine(const MoeArgs& p, const Routed& s, 
     p.out[at] = p.x ? base + v : v;
   }
 }
-template <int QT>
+template <int QT, bool kCluster>
 __global__ void __launch_bounds__(kDownWarps * 32, 1) moe_layer_down_kernel(MoeArgs p) {
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ Routed s;
@@ -501,11 +503,17 @@ __global__ void __launch_bounds__(kDownWarps * 32, 1) moe_layer_down_kernel(MoeA
   const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
   const Copier<QT> copier(p.down_row, lane);
   pdl_launch_next();
-  const int splits_log = p.splits - 1, warps_log = __ffs(warps) - 1, items = route_all(p, s) << splits_log, sbs = p.F / 256, per = p.F / 32;  // (one or two splits)
+  int rank = 0, tile0 = blockIdx.x, tiles = gridDim.x;
+  if (kCluster) asm("mov.u32 %0, %%cluster_ctarank;\n\tmov.u32 %1, %%clusterid.x;\n\tmov.u32 %2, %%nclusterid.x;" : "=r"(rank), "=r"(tile0), "=r"(tiles));
+  tile0 *= 16;
+  tiles *= 16;
+  const int cluster = kCluster ? p.cluster : 1, stride = warps * cluster;
+  if (kCluster) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");  // (waited for before anything is written to another CTA)
+  const int splits_log = p.splits - 1, stride_log = __ffs(stride) - 1, items = route_all(p, s) << splits_log, sbs = p.F / 256, per = p.F / 32;  // (one or two splits)
 
   // what the combine adds to (written before this call's first kernel, so it may be read here)
   float base = 0.0f;
-  if (p.x) base = p.x[min((int)threadIdx.x >> 4, p.T - 1) * p.E + blockIdx.x * 16 + (threadIdx.x & 15)];
+  if (p.x) base = p.x[min((int)threadIdx.x >> 4, p.T - 1) * p.E + tile0 + (threadIdx.x & 15)];
 
   // A place in a warp's work: 16 outputs, an item (an expert's tokens and a part of F: parts of unlike lengths go round among the warps), a superblock.
   struct Place {
@@ -513,22 +521,22 @@ __global__ void __launch_bounds__(kDownWarps * 32, 1) moe_layer_down_kernel(MoeA
   };
   auto open = [&](Place& w) {
     while (w.item >= items && w.n0 < p.E) {
-      w.n0 += gridDim.x * 16;
-      w.item = warp;
+      w.n0 += tiles;
+      w.item = warp * cluster + rank;
       if (w.item >= items) w.n0 = p.E;  // (fewer items than warps)
     }
-    w.k = (w.item + (w.item >> warps_log)) & splits_log;
+    w.k = (w.item + (w.item >> stride_log)) & splits_log;
     w.sb = w.k ? sbs >> 1 : 0;
     w.end = w.k || !splits_log ? sbs : sbs >> 1;
   };
   auto step = [&](Place& w) {
     if (++w.sb == w.end) {
-      w.item += warps;
+      w.item += stride;
       open(w);
     }
   };
-  Place asked = {(int)blockIdx.x * 16, warp, 0, 0, 0};
-  if (warp >= items) asked.n0 = p.E;
+  Place asked = {tile0, warp * cluster + rank, 0, 0, 0};
+  if (asked.item >= items) asked.n0 = p.E;
   open(asked);
   Place now = asked;
   int ask_slot = 0;
@@ -543,6 +551,7 @@ __global__ void __launch_bounds__(kDownWarps * 32, 1) moe_layer_down_kernel(MoeA
 #pragma unroll
   for (int i = 0; i < kSlots; ++i) ask();
   pdl_wait();
+  if (kCluster) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 
   uint2 x[3];
   f2 hs, hm;
@@ -558,7 +567,7 @@ __global__ void __launch_bounds__(kDownWarps * 32, 1) moe_layer_down_kernel(MoeA
     if (Raw<QT>::kMin) hm = *reinterpret_cast<const f2*>(p.hsum + at);
   };
   if (now.n0 < p.E) values(now, __ffs(s.group[now.item >> splits_log]) - 1);
-  for (int n0 = blockIdx.x * 16, slot = 0; n0 < p.E; n0 += gridDim.x * 16) {
+  for (int n0 = tile0, slot = 0; n0 < p.E; n0 += tiles) {
     while (now.n0 == n0) {
       const Place here = now;
       step(now);
@@ -595,12 +604,24 @@ __global__ void __launch_bounds__(kDownWarps * 32, 1) moe_layer_down_kernel(MoeA
         a += __shfl_xor_sync(0xFFFFFFFFu, a, 2);
         if (t < 2) {
           float* to = s_y + ((pair_now << splits_log) + here.k) * 16 + t * 8 + g;
-          *to = first ? a : *to + a;
+          if (!first) a += *to;
+          if (kCluster && here.sb + 1 == here.end) {
+            uint32_t there;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(there) : "r"((uint32_t)__cvta_generic_to_shared(to)));
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(there), "f"(a) : "memory");
+          } else {
+            *to = a;
+          }
         }
       }
     }
-    __syncthreads();
-    down_combine(p, s, s_y, n0, n0 == (int)blockIdx.x * 16, base);
+    if (kCluster) {  // (of one round)
+      asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+      if (rank) break;
+    } else {
+      __syncthreads();
+    }
+    down_combine(p, s, s_y, n0, n0 == tile0, base);
     __syncthreads();
   }
 }
@@ -651,18 +672,26 @@ extern "C" int izb_moe_layer(const izb_weight* wg, const izb_weight* wu, const i
   const int up_grid = units < 2 * sms ? units : 2 * sms;
   // the second kernel: a CTA of 16 warps per multiprocessor, or two of 8 where one round of the former does not do
   const int tiles = E / 16, down_warps = tiles <= sms ? kDownWarps : kDownWarps / 2, most = tiles <= sms ? sms : 2 * sms;
-  const int down_grid = tiles < most ? tiles : most;
+  // (a cluster per 16 outputs while there is a multiprocessor for each CTA and more items, about, than warps: with 14 of them for 32 23 us came to 27)
+  const size_t groups = pairs < wg->n_mats + pairs / kGroup ? pairs : wg->n_mats + pairs / kGroup;
+  p.cluster = 1;
+  while (p.cluster < 8 && tiles * p.cluster * 2 <= sms && groups * p.splits > (size_t)down_warps * p.cluster) p.cluster *= 2;
+  const int down_grid = tiles < most ? tiles * p.cluster : most;
   cudaStream_t st = (cudaStream_t)stream;
   const bool up4 = wg->type == IZB_Q4_K, down4 = wd->type == IZB_Q4_K;
   const size_t up_smem = up4 ? Up<IZB_Q4_K>::kSmem : Up<IZB_Q8_0>::kSmem;
   const size_t down_smem = down4 ? Down<IZB_Q4_K>::smem(down_warps, pairs, p.splits) : Down<IZB_Q8_0>::smem(down_warps, pairs, p.splits);
   IZB_SMEM_OPTIN(moe_layer_up_kernel<IZB_Q4_K>, Up<IZB_Q4_K>::kSmem, wg->device);
   IZB_SMEM_OPTIN(moe_layer_up_kernel<IZB_Q8_0>, Up<IZB_Q8_0>::kSmem, wg->device);
-  IZB_SMEM_OPTIN(moe_layer_down_kernel<IZB_Q4_K>, Down<IZB_Q4_K>::smem(kDownWarps, kMaxPairs, 2), wg->device);
-  IZB_SMEM_OPTIN(moe_layer_down_kernel<IZB_Q8_0>, Down<IZB_Q8_0>::smem(kDownWarps, kMaxPairs, 2), wg->device);
+  IZB_SMEM_OPTIN((moe_layer_down_kernel<IZB_Q4_K, false>), Down<IZB_Q4_K>::smem(kDownWarps, kMaxPairs, 2), wg->device);
+  IZB_SMEM_OPTIN((moe_layer_down_kernel<IZB_Q4_K, true>), Down<IZB_Q4_K>::smem(kDownWarps, kMaxPairs, 2), wg->device);
+  IZB_SMEM_OPTIN((moe_layer_down_kernel<IZB_Q8_0, false>), Down<IZB_Q8_0>::smem(kDownWarps, kMaxPairs, 2), wg->device);
+  IZB_SMEM_OPTIN((moe_layer_down_kernel<IZB_Q8_0, true>), Down<IZB_Q8_0>::smem(kDownWarps, kMaxPairs, 2), wg->device);
   auto up = up4 ? moe_layer_up_kernel<IZB_Q4_K> : moe_layer_up_kernel<IZB_Q8_0>;
-  auto down = down4 ? moe_layer_down_kernel<IZB_Q4_K> : moe_layer_down_kernel<IZB_Q8_0>;
+  const bool shared = p.cluster > 1;
+  auto down = down4 ? (shared ? moe_layer_down_kernel<IZB_Q4_K, true> : moe_layer_down_kernel<IZB_Q4_K, false>)
+                    : (shared ? moe_layer_down_kernel<IZB_Q8_0, true> : moe_layer_down_kernel<IZB_Q8_0, false>);
   IZB_LAUNCH("moe_layer_up", st, izb_launch_pdl(up, up_grid, kUpWarps * 32, up_smem, st, p));
-  IZB_LAUNCH("moe_layer_down", st, izb_launch_pdl(down, down_grid, down_warps * 32, down_smem, st, p));
+  IZB_LAUNCH("moe_layer_down", st, izb_launch_pdl_cluster(down, p.cluster, dim3(down_grid), down_warps * 32, down_smem, st, p));
   return IZB_OK;
 }

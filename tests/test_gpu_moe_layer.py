@@ -242,3 +242,27 @@ def test_refusals(izb, torch):
             izb.moe_layer(*args, 2, **kw)
     with pytest.raises(ValueError):
         izb.moe_layer(*args[:3], b.aq[:, :256], *args[4:], 2)
+
+
+@pytest.mark.parametrize("T,E,F,NE,NU,qt,qd,experts", [
+    (32, 256, 768, 40, 8, 12, 12, None),     # few outputs, many pairs: clusters of eight CTAs
+    (25, 512, 1024, 6, 5, 12, 8, None),
+    (12, 768, 256, 32, 4, 8, 12, (5, 30)),   # some choices are another rank's
+    (32, 1024, 512, 64, 2, 8, 8, (60, 64)),  # hardly any expert is here: most CTAs have nothing to add
+])
+def test_few_outputs_shared_by_a_cluster(izb, torch, T, E, F, NE, NU, qt, qd, experts):
+    b = Block(izb, torch, T, E, F, NE, NU, qt, qd, seed=11, shared=experts is None, experts=experts)
+    want = b.want()
+    got = b.call()
+    assert rel(got, want) <= TOL
+    same = b.x.clone()
+    b.call(x=same, out=same)
+    assert rel(same - b.x, want) <= TOL + 2.0 ** -22 * 8
+    for _ in range(3):
+        assert torch.equal(b.call(), got)
+    # a token's sums do not depend on how many CTAs share them
+    for t in (0, T - 1):
+        asc = torch.zeros((E // 32, 16), device="cuda")
+        asc[:, 0] = b.asc[:, t]
+        one = b.izb.moe_layer(b.wg, b.wu, b.wd, b.aq[t:t + 1].contiguous(), asc, b.logits[t:t + 1].contiguous(), b.NU, sh=b.sh[t:t + 1].contiguous() if b.shared else None, e0=b.e0)
+        assert torch.equal(one[0], got[t])
