@@ -21,6 +21,8 @@
 // that a lane has four neighbouring ones: 16-byte copies of the base and stores.
 #include <cuda_bf16.h>
 
+#include <type_traits>
+
 #include "izb_common.cuh"
 
 namespace {
@@ -763,7 +765,6 @@ template <bool kBf16, int kPlace, bool kRegs>
 __global__ void __launch_bounds__(kThreads, 2) lora_outer_kernel(LoraArgs p, RowsPlan plan, const unsigned char* scratch) {
   extern __shared__ __align__(16) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3, ld = plan.ld;
-  const int m0 = (warp & 3) * 16, half = (warp >> 2) * 32;  // a warp has 16 rows and 32 of the 64 outputs
   const uint32_t smem_at = (uint32_t)__cvta_generic_to_shared(smem), stages_at = smem_at + plan.pieces;
   const bool in_place = p.base == p.C;
   constexpr bool kVec = kPlace == kOnLines;
@@ -780,7 +781,6 @@ __global__ void __launch_bounds__(kThreads, 2) lora_outer_kernel(LoraArgs p, Row
   const int col = kVec ? 4 * (g >> 1) + (g & 1) : g, col_step = kVec ? 2 : 8, out0 = kVec ? 4 * t : 2 * t;
   auto out_of = [&](int k) { return kVec ? k : (k >> 1) * 8 + (k & 1); };
   const int swap = g & 1 ? plan.swap : 0;     // (both columns are as odd as g)
-  auto of_u = [&](int k, int group) { return *reinterpret_cast<const uint4*>(smem + ((k * 4 + (warp & 3)) * (ld / 16) + group) * 512 + lane * 16); };
   const int b_row = tid >> 2, b_chunk = tid & 3;  // four threads copy a row of B
   const uint32_t b_to = stages_at + (b_row * ld + (b_chunk ^ (b_row & 1 ? plan.swap : 0)) * 8) * 2, b_swap = b_row & 1 && plan.swap ? 0xFFFFFFC0u : 64u;  // (the next four chunks)
   const uint32_t base_to = stages_at + kCols * ld * 2 + (kPlace == kAlike ? (b_row * kPitch + b_chunk * 4) * 4 : tid * 16);
@@ -790,6 +790,11 @@ __global__ void __launch_bounds__(kThreads, 2) lora_outer_kernel(LoraArgs p, Row
   int index = (int)(begin / per), step0 = (int)(begin % per);
   for (long long left = end - begin; left > 0; ++index, step0 = 0) {
     const Tile tile = tiles[index];
+    // A warp has 16 rows and 32 of the 64 outputs; of a tile of 32 rows or fewer 16 outputs, so that all four tensor cores have work (42 segments of 9 rows,
+    // 3840 -> 11281 at rank 128: 110 us against 129; 16 of 16, 5120 -> 17408 at rank 64: 32 against 38)
+    const bool narrow = tile.rows <= 32;
+    const int m0 = (narrow ? warp >> 2 : warp & 3) * 16, half = narrow ? (warp & 3) * 16 : (warp >> 2) * 32;
+    auto of_u = [&](int k, int group) { return *reinterpret_cast<const uint4*>(smem + ((k * 4 + (m0 >> 4)) * (ld / 16) + group) * 512 + lane * 16); };
     const int steps = (int)min(left, (long long)(per - step0)), rank = (tile.rank + 15) & ~15;
     left -= steps;
     if (in_place && rank == 0) continue;
@@ -845,7 +850,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_outer_kernel(LoraArgs p, Row
           for (int c = 0; c < mine; ++c) copy16(b_to + ask_at + (c >> 1) * 128 + (c & 1 ? b_swap : 0u), from + 32 * c);
         }
         b_from += (size_t)kCols * p.R;
-        if (p.base) {
+        if (p.base && (kPlace == kAlike || m0 < tile.rows)) {
           const uint32_t to = base_to + ask_at;
           if (kPlace == kAlike) {
 #pragma unroll
@@ -863,8 +868,10 @@ __global__ void __launch_bounds__(kThreads, 2) lora_outer_kernel(LoraArgs p, Row
           } else if (kVec && ask_n + kCols <= p.N) {
             copy16(to, from0);
             copy16(to + kThreads * 16, from1);
-            copy16(to + 2 * kThreads * 16, from0 + 16);
-            copy16(to + 3 * kThreads * 16, from1 + 16);
+            if (!narrow) {
+              copy16(to + 2 * kThreads * 16, from0 + 16);
+              copy16(to + 3 * kThreads * 16, from1 + 16);
+            }
           } else {
             const int n = ask_n + half + out0;
 #pragma unroll
@@ -873,7 +880,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_outer_kernel(LoraArgs p, Row
                 copy4(to + k * 4, from0 + out_of(k));
                 copy4(to + kThreads * 16 + k * 4, from1 + out_of(k));
               }
-              if (n + 16 + out_of(k) < p.N) {
+              if (!narrow && n + 16 + out_of(k) < p.N) {
                 copy4(to + 2 * kThreads * 16 + k * 4, from0 + 16 + out_of(k));
                 copy4(to + 3 * kThreads * 16 + k * 4, from1 + 16 + out_of(k));
               }
@@ -941,95 +948,100 @@ __global__ void __launch_bounds__(kThreads, 2) lora_outer_kernel(LoraArgs p, Row
       here += plan.stage2;
       if (here == smem + plan.pieces + stages_end) here = smem + plan.pieces;
       if (m0 >= tile.rows) continue;
-      float d[2][2][4] = {};
-      // chunks of 32 ranks of B's rows: sixteen outputs h, instruction q
-      auto of_b = [&](int h, int q, int chunk) { return b + (16 * h + col_step * q) * ld + (chunk ^ swap) * 8; };
-      if (kRegs) {
+      auto outputs = [&](auto sixteens) {
+        constexpr int kH = decltype(sixteens)::value;
+        float d[kH][2][4] = {};
+        // chunks of 32 ranks of B's rows: sixteen outputs h, instruction q
+        auto of_b = [&](int h, int q, int chunk) { return b + (16 * h + col_step * q) * ld + (chunk ^ swap) * 8; };
+        if (kRegs) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          if (32 * j + 32 <= rank) {
+          for (int j = 0; j < 2; ++j) {
+            if (32 * j + 32 <= rank) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+              for (int h = 0; h < kH; ++h)
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                  const uint4 v = *reinterpret_cast<const uint4*>(of_b(h, q, 4 * j));
+#pragma unroll
+                  for (int k = 0; k < kPieces<kBf16>; ++k) mma32<kBf16>(d[h][q], held[kRegs ? j : 0][k][0], held[kRegs ? j : 0][k][1], v);
+                }
+            }
+          }
+        }
+        int j = kRegs ? rank & ~31 : 0;
+        if (!kRegs)
+          for (; j + 32 <= rank; j += 32) {
+            uint4 v[kH][2];
+#pragma unroll
+            for (int h = 0; h < kH; ++h)
+#pragma unroll
+              for (int q = 0; q < 2; ++q) v[h][q] = *reinterpret_cast<const uint4*>(of_b(h, q, j / 8));
+#pragma unroll
+            for (int k = 0; k < kPieces<kBf16>; ++k) {
+              const uint4 r0 = of_u(k, j / 16), r1 = of_u(k, j / 16 + 1);
+#pragma unroll
+              for (int h = 0; h < kH; ++h)
+#pragma unroll
+                for (int q = 0; q < 2; ++q) mma32<kBf16>(d[h][q], r0, r1, v[h][q]);
+            }
+          }
+        if (j < rank) {  // sixteen more: a lane has four of them, in chunk t / 2 of the two
+          const int at = (j / 8 ^ swap) * 8 + 4 * t - 8 * t;
+#pragma unroll
+          for (int k = 0; k < kPieces<kBf16>; ++k) {
+            const uint4 r = of_u(k, j / 16);
+#pragma unroll
+            for (int h = 0; h < kH; ++h)
 #pragma unroll
               for (int q = 0; q < 2; ++q) {
-                const uint4 v = *reinterpret_cast<const uint4*>(of_b(h, q, 4 * j));
-#pragma unroll
-                for (int k = 0; k < kPieces<kBf16>; ++k) mma32<kBf16>(d[h][q], held[kRegs ? j : 0][k][0], held[kRegs ? j : 0][k][1], v);
+                const uint2 v = *reinterpret_cast<const uint2*>(b + (16 * h + col_step * q) * ld + at);
+                mma<kBf16>(d[h][q], r.x, r.y, r.z, r.w, v.x, v.y);
               }
           }
         }
-      }
-      int j = kRegs ? rank & ~31 : 0;
-      if (!kRegs)
-        for (; j + 32 <= rank; j += 32) {
-          uint4 v[2][2];
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int q = 0; q < 2; ++q) v[h][q] = *reinterpret_cast<const uint4*>(of_b(h, q, j / 8));
-#pragma unroll
-          for (int k = 0; k < kPieces<kBf16>; ++k) {
-            const uint4 r0 = of_u(k, j / 16), r1 = of_u(k, j / 16 + 1);
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-              for (int q = 0; q < 2; ++q) mma32<kBf16>(d[h][q], r0, r1, v[h][q]);
-          }
-        }
-      if (j < rank) {  // sixteen more: a lane has four of them, in chunk t / 2 of the two
-        const int at = (j / 8 ^ swap) * 8 + 4 * t - 8 * t;
-#pragma unroll
-        for (int k = 0; k < kPieces<kBf16>; ++k) {
-          const uint4 r = of_u(k, j / 16);
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              const uint2 v = *reinterpret_cast<const uint2*>(b + (16 * h + col_step * q) * ld + at);
-              mma<kBf16>(d[h][q], r.x, r.y, r.z, r.w, v.x, v.y);
+        for (int h = 0; h < kH; ++h) {
+          float4 o0 = make_float4(0.0f, 0.0f, 0.0f, 0.0f), o1 = o0;
+          float *s0 = nullptr, *s1 = nullptr;
+          if (kPlace == kAlike) {
+            float* line = const_cast<float*>(reinterpret_cast<const float*>(stage + kCols * ld * 2)) + 16 * h;
+            s0 = line + at0;
+            s1 = line + at1;
+            if (p.base) {
+              o0 = make_float4(s0[out_of(0)], s0[out_of(1)], s0[out_of(2)], s0[out_of(3)]);
+              o1 = make_float4(s1[out_of(0)], s1[out_of(1)], s1[out_of(2)], s1[out_of(3)]);
             }
-        }
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float4 o0 = make_float4(0.0f, 0.0f, 0.0f, 0.0f), o1 = o0;
-        float *s0 = nullptr, *s1 = nullptr;
-        if (kPlace == kAlike) {
-          float* line = const_cast<float*>(reinterpret_cast<const float*>(stage + kCols * ld * 2)) + 16 * h;
-          s0 = line + at0;
-          s1 = line + at1;
-          if (p.base) {
-            o0 = make_float4(s0[out_of(0)], s0[out_of(1)], s0[out_of(2)], s0[out_of(3)]);
-            o1 = make_float4(s1[out_of(0)], s1[out_of(1)], s1[out_of(2)], s1[out_of(3)]);
+          } else if (p.base) {
+            o0 = old[2 * h * kThreads];
+            o1 = old[(2 * h + 1) * kThreads];
           }
-        } else if (p.base) {
-          o0 = old[2 * h * kThreads];
-          o1 = old[(2 * h + 1) * kThreads];
-        }
-        if (rank) {
-          o0 = make_float4(fmaf(f0, d[h][0][0], o0.x), fmaf(f0, d[h][0][1], o0.y), fmaf(f0, d[h][1][0], o0.z), fmaf(f0, d[h][1][1], o0.w));
-          o1 = make_float4(fmaf(f1, d[h][0][2], o1.x), fmaf(f1, d[h][0][3], o1.y), fmaf(f1, d[h][1][2], o1.z), fmaf(f1, d[h][1][3], o1.w));
-        }
-        if (kPlace == kAlike) {
-          const float v0[4] = {o0.x, o0.y, o0.z, o0.w}, v1[4] = {o1.x, o1.y, o1.z, o1.w};
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            s0[out_of(k)] = v0[k];
-            s1[out_of(k)] = v1[k];
+          if (rank) {
+            o0 = make_float4(fmaf(f0, d[h][0][0], o0.x), fmaf(f0, d[h][0][1], o0.y), fmaf(f0, d[h][1][0], o0.z), fmaf(f0, d[h][1][1], o0.w));
+            o1 = make_float4(fmaf(f1, d[h][0][2], o1.x), fmaf(f1, d[h][0][3], o1.y), fmaf(f1, d[h][1][2], o1.z), fmaf(f1, d[h][1][3], o1.w));
           }
-        } else if (kVec && n - half - out0 + kCols <= p.N) {
-          if (has0) *reinterpret_cast<float4*>(c0 + 16 * h) = o0;
-          if (has1) *reinterpret_cast<float4*>(c1 + 16 * h) = o1;
-        } else {
-          const float v0[4] = {o0.x, o0.y, o0.z, o0.w}, v1[4] = {o1.x, o1.y, o1.z, o1.w};
+          if (kPlace == kAlike) {
+            const float v0[4] = {o0.x, o0.y, o0.z, o0.w}, v1[4] = {o1.x, o1.y, o1.z, o1.w};
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (n + 16 * h + out_of(k) < p.N) {
-              if (has0) c0[16 * h + out_of(k)] = v0[k];
-              if (has1) c1[16 * h + out_of(k)] = v1[k];
+            for (int k = 0; k < 4; ++k) {
+              s0[out_of(k)] = v0[k];
+              s1[out_of(k)] = v1[k];
             }
+          } else if (kVec && n - half - out0 + kCols <= p.N) {
+            if (has0) *reinterpret_cast<float4*>(c0 + 16 * h) = o0;
+            if (has1) *reinterpret_cast<float4*>(c1 + 16 * h) = o1;
+          } else {
+            const float v0[4] = {o0.x, o0.y, o0.z, o0.w}, v1[4] = {o1.x, o1.y, o1.z, o1.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (n + 16 * h + out_of(k) < p.N) {
+                if (has0) c0[16 * h + out_of(k)] = v0[k];
+                if (has1) c1[16 * h + out_of(k)] = v1[k];
+              }
+          }
         }
-      }
+      };
+      if (narrow) outputs(std::integral_constant<int, 1>());
+      else outputs(std::integral_constant<int, 2>());
     }
     copies_there<0>();
     if (kPlace == kAlike) {
