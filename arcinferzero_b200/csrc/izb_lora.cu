@@ -11,8 +11,7 @@
 // four rows, rank 32: 34 (9.2); 8192 rows, ranks 64 and 32, 5120 -> 17408: 250 (182), of which the second product 205 at 5.8 TB/s.
 //
 // Two forms.  Decode rows (lora_few_kernel, up to 8 rows per segment on average): one launch and no memory for u.  A cluster of CTAs per tile of up to 8 rows
-// of a segment, each with a share of K; the partial sums meet in distributed shared memory, and each CTA goes on with its share of the outputs.  Ranks, then
-// outputs, are on the instruction's 16-wide side and rows on the 8-wide one.
+// of a segment, each with a share of K; the partial sums meet in distributed shared memory, and each CTA goes on with its share of the outputs.
 // What bounds it is a chain: which rows, the adapter's first bytes, the exchange of sums (2 + 5 + 2 us), then B.  A call where every request has one row
 // takes tiles of one row (lora_few_kernel<.., 1>): less shared memory, three CTAs per multiprocessor, the second product in plain f32.
 // Prompts: tiles of up to 64 rows.  lora_inner_kernel makes u's pieces (a cluster per tile, a share of K each) and a list of the tiles; lora_outer_kernel
@@ -616,7 +615,7 @@ struct RowsPlan {
   size_t scratch(size_t tiles) const { return at_pieces + tiles * pieces; }
 };
 // The first product: u's pieces, rows' factors and the tile's place, into scratch.
-template <bool kBf16>
+template <bool kBf16, int kParts>
 __global__ void __launch_bounds__(kThreads, 2) lora_inner_kernel(LoraArgs p, RowsPlan plan, unsigned char* scratch) {
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ Tile s_tile;
@@ -642,26 +641,30 @@ __global__ void __launch_bounds__(kThreads, 2) lora_inner_kernel(LoraArgs p, Row
   const int rank = (tile.rank + 15) & ~15;
 
   // ---- a warp has 64 ranks x 32 rows, and every parts-th 32-block of the CTA's share of K; `parts` blocks per stage
-  const int parts = plan.parts, part = warp % parts, r0 = (warp / parts & 1) * 32, j0 = warp / (2 * parts) * 64;
+  constexpr int parts = kParts;
+  const int part = warp % parts, r0 = (warp / parts & 1) * 32, j0 = warp / (2 * parts) * 64;
   {
     const int kb0 = share(p.K / 32, p.cluster, rank_of_cta), kb1 = share(p.K / 32, p.cluster, rank_of_cta + 1), steps = (kb1 - kb0 + parts - 1) / parts;
-    const int row_log = __ffs(parts) + 1, swap = parts > 1 ? 4 : 0;  // a row of A's tile: 2^row_log chunks
+    constexpr int row_log = parts == 4 ? 4 : parts == 2 ? 3 : 2, swap = parts > 1 ? 4 : 0;  // a row of A's tile: 2^row_log chunks
     const uint32_t stages_at = (uint32_t)__cvta_generic_to_shared(smem), scales_at = parts * kRows * 32, a_at = scales_at + parts * kRows * 4;
     // (rows past the tile's: the last one again, which nobody reads)
     const int8_t* x_from = p.aq + (size_t)(tile.row + min((tid >> 1) & (kRows - 1), tile.rows - 1)) * p.K + (kb0 + (tid >> 7)) * 32 + (tid & 1) * 16;
     const float* s_from = p.asc + (size_t)(kb0 + (tid >> 6)) * p.Mp + tile.row + min(tid & (kRows - 1), tile.rows - 1);
     const int a_c = tid & ((1 << row_log) - 1), a_j = tid >> row_log, a_step = kThreads >> row_log;
     const uint16_t* a_from = A + (size_t)a_j * p.K + kb0 * 32 + a_c * 8;
+    const size_t a_rows = (size_t)a_step * p.K;
     const uint32_t a_to = a_at + ((a_j << row_log) + (a_c ^ (a_j & 1 ? swap : 0))) * 16;  // (a_step is even: the rows of a thread are all odd or all even)
     auto ask = [&](int step, int stage) {
       if (step < steps) {
         const uint32_t to = stages_at + stage * plan.stage1;
         const int blocks = min(parts, kb1 - kb0 - step * parts), k = step * parts * 32;
-        for (int i = tid; i < blocks * kRows * 2; i += kThreads) copy16(to + i * 16, x_from + k + (i - tid) / 4);
+#pragma unroll
+        for (int i = 0; i < parts * kRows * 2; i += kThreads)
+          if (tid + i < blocks * kRows * 2) copy16(to + (tid + i) * 16, x_from + k + i / 4);
         if (tid < blocks * kRows) copy4(to + scales_at + tid * 4, s_from + (size_t)(step * parts) * p.Mp);
         if (a_c < blocks * 4) {
           const uint16_t* from = a_from + k;
-          for (int j = a_j, i = 0; j < rank; j += a_step, ++i, from += (size_t)a_step * p.K) copy16(to + a_to + i * (kThreads * 16), from);
+          for (int j = a_j, i = 0; j < rank; j += a_step, ++i, from += a_rows) copy16(to + a_to + i * (kThreads * 16), from);
         }
       }
       copies_begun();
@@ -1112,8 +1115,11 @@ extern "C" int izb_lora_add(int dtype, const void* d_A, const void* d_B, int n_a
   const bool vec = izb_aligned(p.C, 16) && ldc % 4 == 0 && (!d_base || (izb_aligned(d_base, 16) && ldb % 4 == 0));
   const int place = vec ? kOnLines : !d_base || (((uintptr_t)p.C - (uintptr_t)d_base) % 16 == 0 && (ldc - (int64_t)ldb) % 4 == 0) ? kAlike : kAnywhere;
   const RowsPlan plan(R, bf16, tiles, place);
-  static izb_device_once once[14];
-  void (*const inner)(LoraArgs, RowsPlan, unsigned char*) = bf16 ? lora_inner_kernel<true> : lora_inner_kernel<false>;
+  static izb_device_once once[18];
+  void (*const inners[6])(LoraArgs, RowsPlan, unsigned char*) = {lora_inner_kernel<false, 1>, lora_inner_kernel<false, 2>, lora_inner_kernel<false, 4>,
+                                                                 lora_inner_kernel<true, 1>, lora_inner_kernel<true, 2>, lora_inner_kernel<true, 4>};
+  const int which_inner = (bf16 ? 3 : 0) + plan.parts / 2;
+  auto inner = inners[which_inner];
   void (*const outers[12])(LoraArgs, RowsPlan, const unsigned char*) = {
       lora_outer_kernel<false, kOnLines, false>, lora_outer_kernel<false, kOnLines, true>, lora_outer_kernel<false, kAlike, false>, lora_outer_kernel<false, kAlike, true>,
       lora_outer_kernel<false, kAnywhere, false>, lora_outer_kernel<false, kAnywhere, true>, lora_outer_kernel<true, kOnLines, false>, lora_outer_kernel<true, kOnLines, true>,
@@ -1124,7 +1130,7 @@ extern "C" int izb_lora_add(int dtype, const void* d_A, const void* d_B, int n_a
         return IZB_OK;
       }))
     return rc;
-  if (int rc = once[12 + bf16].run(device, [&]() -> int {
+  if (int rc = once[12 + which_inner].run(device, [&]() -> int {
         IZB_CUDA(cudaFuncSetAttribute(inner, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxInner));
         IZB_CUDA(cudaFuncSetAttribute(inner, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
         return IZB_OK;
