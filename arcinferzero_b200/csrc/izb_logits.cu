@@ -16,7 +16,8 @@
 // most of it belongs to others: handing tokens on through distributed shared memory would save less than the cluster-wide barrier costs.  Rows with more than
 // 65535 of either take two words per token and half the window at a time.
 // (Taken back: a bitmap of the tokens that the rules touch, and counts for those alone, numbered by its running sum.  The pass over the others is then
-// free of rules, but the steps before it wait for memory one after the other: 64 rows 55 us against 36.  The touched tokens of a lane one by one instead of its
+// free of rules, but the steps before it wait for memory one after the other: 64 rows that stay in L2 55 us against 36.  Counts of 16 bits, two to a word, with biases
+// marked and looked up in their list: 71 against 41.  The touched tokens of a lane one by one instead of its
 // four together: 93 against 85 for 256 rows, by the registers it takes.)
 #include <math.h>
 

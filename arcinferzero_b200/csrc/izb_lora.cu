@@ -8,7 +8,7 @@
 // would want 128 rows of one adapter per tile and its accumulators back through registers for the base; the tensor pipe is 46 % busy at most.)
 //
 // Measured (us; floor by bytes): one row of 5120 -> 5120, rank 16: 5.0 (0.06); 64 requests of one row, 32 adapters of ranks 8 to 64, 5120 -> 17408: 29 (8.0); 64 of
-// four rows, rank 32: 34 (9.2); 8192 rows, ranks 64 and 32, 5120 -> 17408: 250 (182), of which the second product 205 at 5.8 TB/s.
+// four rows, rank 32: 34 (9.2); 8192 rows, ranks 64 and 32, 5120 -> 17408: 245 (182), of which the second product 205 at 5.5 TB/s.
 //
 // Two forms.  Decode rows (lora_few_kernel, up to 8 rows per segment on average): one launch and no memory for u.  A cluster of CTAs per tile of up to 8 rows
 // of a segment, each with a share of K; the partial sums meet in distributed shared memory, and each CTA goes on with its share of the outputs.
@@ -1093,7 +1093,7 @@ extern "C" int izb_lora_add(int dtype, const void* d_A, const void* d_B, int n_a
   if (one) p.cluster = kFewBlocks<1> * sms / T > widest ? widest : kFewBlocks<1> * sms / T < 4 ? 4 : kFewBlocks<1> * sms / T;
   else p.cluster = few && n_seg * 16ll <= 2 * sms ? widest : 8;
   if (!few)
-    for (p.cluster = 16; p.cluster > 1 && (T / kRows + (n_seg + 1ll) / 2) * p.cluster > 2 * sms;) p.cluster /= 2;
+    for (p.cluster = widest; p.cluster > 1 && (T / kRows + (n_seg + 1ll) / 2) * p.cluster > 2 * sms;) p.cluster /= 2;
   if (tiles * p.cluster > 0x7FFFFFFF) IZB_FAIL(IZB_ERR_LIMIT, "lora_add: %d rows in %d segments", T, n_seg);
   const dim3 grid((unsigned)(tiles * p.cluster));
   if (few) {

@@ -17,7 +17,7 @@
 // and asks for its first weights while the first kernel still runs.
 //
 // Measured (us; the six calls / this; the floor by bytes), 128 experts of 768 over 2048, top 8, Q4_K: one token 26 / 18 (3.3), four 48 / 36, eight 88 / 55 (21),
-// 16 154 / 88, 32 208 / 147 (45); 60 experts of 1280 over 4096, top 4, five tokens 99 / 56.  Many tokens per expert are where the block-per-column form has nothing
+// 16 154 / 88, 32 208 / 143 (45); 60 experts of 1280 over 4096, top 4, five tokens 99 / 56.  Many tokens per expert are where the block-per-column form has nothing
 // to gain (it costs every token eight instructions): 8 experts, top 2, 32 tokens 47 / 55.  One token is latency: routing 2.6 us, first bytes of weights 2.4, the
 // barriers.  Eight tokens: the first kernel's loop runs at 4.1 TB/s, the second one's at 2.9, both near 48 % of the issue slots with 16 warps per multiprocessor:
 // a superblock of gate and up takes about 560 instructions, of which decoding 6-bit scales is a fifth.
