@@ -156,7 +156,8 @@ int izb_workspace(int device, int slot, size_t bytes, cudaStream_t st, void** ou
 // A decode step is a chain of kernels of a few microseconds, each waiting for the one before.  Launched with this attribute
 // a kernel's CTAs move in as soon as every CTA of the kernel before it has called pdl_launch_next() (or ended) and room is
 // free; it may set itself up and touch what no kernel writes (the library's weights), and calls pdl_wait() -- which returns
-// when the kernel before it has completed and its writes are visible -- before it reads or writes anything else.  Every
+// when the kernel before it has completed and its writes are visible -- before it reads or writes anything else: pdl_launch_next() makes
+// nothing visible, not even what kernels before that one wrote, however early its own wait.  Every
 // kernel launched this way calls pdl_wait() on every path, so completion stays transitive along the stream.
 //
 // izb_one_wave: does a grid of such blocks fit the current device at once (2048 threads per SM)?  Short blocks of many waves are faster without

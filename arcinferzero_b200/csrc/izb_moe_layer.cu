@@ -12,9 +12,9 @@
 // column b and zeros beside them, eight instructions add up to the 16 x 8 block sums, and lane t scales blocks 2t and 2t + 1 of its two rows -- each
 // scale is decoded by one lane, once.  What comes after is a sum over the quad.
 //
-// Routing is done by every CTA for itself (a warp per token; 2.6 us, with what follows from it, against a launch and its hand-over).  The first kernel lets the
-// second one in behind its own wait for the kernel before: what was written before this call is then visible to the second kernel from its start, and it routes
-// and asks for its first weights while the first kernel still runs.
+// Routing is done by every CTA of the first kernel for itself (a warp per token; 2.6 us, with what follows from it, against a launch and its hand-over); one of
+// them writes it out for the second kernel, which reads it behind its wait for the first one: what kernels before this call wrote is visible to it from
+// there on only.
 //
 // Measured (us; the six calls / this; the floor by bytes), 128 experts of 768 over 2048, top 8, Q4_K: one token 26 / 18 (3.3), four 48 / 36, eight 88 / 55 (21),
 // 16 154 / 88, 32 208 / 143 (45); 60 experts of 1280 over 4096, top 4, five tokens 99 / 56.  Many tokens per expert are where the block-per-column form has nothing
@@ -39,6 +39,7 @@ struct MoeArgs {
   const float *asc, *logits, *x, *sh;
   int8_t* hq;         // [T * NU][3][F]
   float *hs, *hsum;   // [T * NU][F / 32]: the power of two, the sum of the block's values
+  uint32_t* routes;   // the routing, as write_routes leaves it
   float* out;
   int T, Mp, ldl, NE, NU, e0, n_mats, E, F, joined, splits, cluster;
   size_t gate_row, down_row;  // bytes of a row
@@ -48,14 +49,16 @@ struct MoeArgs {
 struct Routed {
   float wt[kMaxPairs];
   short id[kMaxPairs];           // the expert's number in the stacks, -1: not here
-  uint32_t tokens[kMaxExperts];  // of an expert
   short list[kMaxPairs];         // experts with tokens, in increasing order, once per kGroup of them ...
   uint32_t group[kMaxPairs];     // ... and which those are
+};
+struct Routing : Routed {
+  uint32_t tokens[kMaxExperts];  // of an expert
   int count[16];
 };
 // One warp: a token's choices in order, ties to the lower id (see izb_moe.cu); the weights' sum in choice order.
 template <int kPer>
-__device__ __forceinline__ void route_token(const MoeArgs& p, int token, Routed& s) {
+__device__ __forceinline__ void route_token(const MoeArgs& p, int token, Routing& s) {
   const int lane = threadIdx.x & 31;
   const float* row = p.logits + (size_t)token * p.ldl;
   uint32_t key[kPer];
@@ -106,7 +109,7 @@ __device__ __forceinline__ void route_token(const MoeArgs& p, int token, Routed&
   }
 }
 // All tokens; the length of the list.  Every thread of the CTA calls it.
-__device__ __forceinline__ int route_all(const MoeArgs& p, Routed& s) {
+__device__ __forceinline__ int route_all(const MoeArgs& p, Routing& s) {
   const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5, lane = threadIdx.x & 31;
   for (int i = threadIdx.x; i < kMaxExperts; i += blockDim.x) s.tokens[i] = 0u;
   __syncthreads();
@@ -144,6 +147,34 @@ __device__ __forceinline__ int route_all(const MoeArgs& p, Routed& s) {
   }
   __syncthreads();
   return n;
+}
+// The routing of T * NU pairs in memory: the length of the list (and three words of nothing) | weights | experts | the list | its tokens.
+__device__ __forceinline__ void write_routes(const MoeArgs& p, const Routed& s, int entries) {
+  const int pairs = p.T * p.NU;
+  if (threadIdx.x == 0) p.routes[0] = (uint32_t)entries;
+  uint32_t* to = p.routes + 4;
+  for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
+    to[i] = __float_as_uint(s.wt[i]);
+    to[pairs + i] = (uint32_t)s.id[i];
+    if (i < entries) {
+      to[2 * pairs + i] = (uint32_t)s.list[i];
+      to[3 * pairs + i] = s.group[i];
+    }
+  }
+}
+// Every thread of the CTA calls it; the length of the list.
+__device__ __forceinline__ int read_routes(const MoeArgs& p, Routed& s) {
+  const int pairs = p.T * p.NU, entries = (int)p.routes[0];
+  const uint32_t* from = p.routes + 4;
+  for (int i = threadIdx.x; i < pairs; i += blockDim.x) {  // (behind the list's end: what is there, unused)
+    const uint32_t wt = from[i], id = from[pairs + i], list = from[2 * pairs + i], group = from[3 * pairs + i];
+    s.wt[i] = __uint_as_float(wt);
+    s.id[i] = (short)id;
+    s.list[i] = (short)list;
+    s.group[i] = group;
+  }
+  __syncthreads();
+  return entries;
 }
 // which of its choices expert `e` is for `token`, as a pair number
 __device__ __forceinline__ int pair_of(const MoeArgs& p, const Routed& s, int token, int e) {
@@ -343,7 +374,7 @@ __device__ __forceinline__ void up_epilogue(const MoeArgs& p, const Routed& s, c
 template <int QT>
 __global__ void __launch_bounds__(kUpWarps * 32, 2) moe_layer_up_kernel(MoeArgs p) {
   extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ Routed s;
+  __shared__ Routing s;
   constexpr int kSlots = Up<QT>::kSlots, kSlot = Up<QT>::kSlot;
   auto s_sum = reinterpret_cast<float(*)[kUpWarps][kGroup][32]>(smem);  // [two units][..][..][gate row, up row of the warp]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, half = warp / kSplitK, part = warp % kSplitK;
@@ -353,6 +384,7 @@ __global__ void __launch_bounds__(kUpWarps * 32, 2) moe_layer_up_kernel(MoeArgs 
   pdl_wait();
   pdl_launch_next();
   const int sbs = p.E / 256, entries = route_all(p, s);
+  if (blockIdx.x == 0) write_routes(p, s, entries);
 
   // A unit is an entry of the list and a block of 32 channels; a CTA takes every gridDim.x-th.
   struct Unit {
@@ -509,9 +541,11 @@ __global__ void __launch_bounds__(kDownWarps * 32, 1) moe_layer_down_kernel(MoeA
   tiles *= 16;
   const int cluster = kCluster ? p.cluster : 1, stride = warps * cluster;
   if (kCluster) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");  // (waited for before anything is written to another CTA)
-  const int splits_log = p.splits - 1, stride_log = __ffs(stride) - 1, items = route_all(p, s) << splits_log, sbs = p.F / 256, per = p.F / 32;  // (one or two splits)
+  const int splits_log = p.splits - 1, stride_log = __ffs(stride) - 1, sbs = p.F / 256, per = p.F / 32;  // (one or two splits)
+  pdl_wait();
+  const int items = read_routes(p, s) << splits_log;
 
-  // what the combine adds to (written before this call's first kernel, so it may be read here)
+  // what the combine adds to
   float base = 0.0f;
   if (p.x) base = p.x[min((int)threadIdx.x >> 4, p.T - 1) * p.E + tile0 + (threadIdx.x & 15)];
 
@@ -550,7 +584,6 @@ __global__ void __launch_bounds__(kDownWarps * 32, 1) moe_layer_down_kernel(MoeA
   };
 #pragma unroll
   for (int i = 0; i < kSlots; ++i) ask();
-  pdl_wait();
   if (kCluster) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 
   uint2 x[3];
@@ -631,8 +664,8 @@ bool takes(const izb_weight* w) { return w->type == IZB_Q4_K || w->type == IZB_Q
 }  // namespace
 
 extern "C" size_t izb_moe_layer_scratch(int T, int NU, int F) {
-  // three digits of every value of h, a scale and a sum per 32 of them
-  return T < 1 || NU < 1 || F < 1 ? 0 : (size_t)T * NU * ((size_t)F * 3 + (size_t)F / 32 * 8);
+  // three digits of every value of h, a scale and a sum per 32 of them; the routing
+  return T < 1 || NU < 1 || F < 1 ? 0 : (size_t)T * NU * ((size_t)F * 3 + (size_t)F / 32 * 8 + 16) + 16;
 }
 
 extern "C" int izb_moe_layer(const izb_weight* wg, const izb_weight* wu, const izb_weight* wd, const int8_t* d_aq, const float* d_asc, int T, int Mp,
@@ -664,6 +697,7 @@ extern "C" int izb_moe_layer(const izb_weight* wg, const izb_weight* wu, const i
   p.aq = d_aq; p.asc = d_asc; p.logits = d_logits; p.x = d_x; p.sh = d_sh;
   const size_t pairs = (size_t)T * NU;
   p.hq = (int8_t*)d_scratch; p.hs = (float*)((int8_t*)d_scratch + pairs * 3 * F); p.hsum = p.hs + pairs * (F / 32);
+  p.routes = (uint32_t*)(p.hsum + pairs * (F / 32));
   p.out = d_out;
   p.T = T; p.Mp = Mp; p.ldl = ldl; p.NE = NE; p.NU = NU; p.e0 = e0; p.n_mats = wg->n_mats; p.E = E; p.F = F;
   p.joined = wg->gu32; p.gate_row = wg->row_bytes; p.down_row = wd->row_bytes;
