@@ -685,7 +685,7 @@ extern "C" int izb_moe_layer(const izb_weight* wg, const izb_weight* wu, const i
   if (T > kMaxTokens || T * NU > kMaxPairs)
     IZB_FAIL(IZB_ERR_LIMIT, "moe_layer: %d tokens x %d experts (up to %d tokens and %d pairs: izb_moe_route, _sort, _gateup, _down and _combine take more)", T, NU, kMaxTokens, kMaxPairs);
   if (!d_scratch) IZB_FAIL(IZB_ERR_ARG, "moe_layer: no scratch");
-  if (e0 < 0 || e0 + wg->n_mats > NE) IZB_FAIL(IZB_ERR_SHAPE, "moe_layer: experts [%d, %d) of %d", e0, e0 + wg->n_mats, NE);
+  if (e0 < 0 || e0 > NE - wg->n_mats) IZB_FAIL(IZB_ERR_SHAPE, "moe_layer: %d experts from %d on, of %d", wg->n_mats, e0, NE);
   if (!izb_aligned(d_aq, 16) || !izb_aligned(d_scratch, 16)) IZB_FAIL(IZB_ERR_ALIGN, "moe_layer: aq and scratch must be 16-byte aligned");
   if (!izb_aligned(d_asc, 4) || !izb_aligned(d_logits, 4) || !izb_aligned(d_out, 4) || !izb_aligned(d_x, 4) || !izb_aligned(d_sh, 4))
     IZB_FAIL(IZB_ERR_ALIGN, "moe_layer: f32 pointers must be 4-byte aligned");

@@ -266,3 +266,12 @@ def test_few_outputs_shared_by_a_cluster(izb, torch, T, E, F, NE, NU, qt, qd, ex
         asc[:, 0] = b.asc[:, t]
         one = b.izb.moe_layer(b.wg, b.wu, b.wd, b.aq[t:t + 1].contiguous(), asc, b.logits[t:t + 1].contiguous(), b.NU, sh=b.sh[t:t + 1].contiguous() if b.shared else None, e0=b.e0)
         assert torch.equal(one[0], got[t])
+
+
+def test_refuses_a_first_expert_that_no_sum_holds(izb, torch):
+    """e0 + n_mats past 2^31."""
+    b = Block(izb, torch, 2, 256, 256, 4, 2, 12, 12)
+    for e0 in (2 ** 31 - 1, 2 ** 31 - 4, 5):
+        with pytest.raises(izb.IzbError) as e:
+            izb.moe_layer(b.wg, b.wu, b.wd, b.aq, b.asc, b.logits, 2, x=b.x, e0=e0)
+        assert e.value.status == -2
