@@ -1,8 +1,9 @@
 // The whole mixture-of-experts block of a few tokens (a decode step's) in two kernels: routing, gate and up projections with SwiGLU, then the
 // down projection with the weighted sum over a token's experts, the shared expert's output and the residual.
 //   e_k, w_k as izb_moe_route;  g = x Wg_e^T, u = x Wu_e^T;  h = u * g / (1 + exp(-g));  out = x + sum_k w_k h_k Wd_e^T + sgate * sh
-// The six-call path quantises h to int8 in between; here a block of 32 values of h is 23-bit integers Q times a power of two, in three int8 digits
-// (Q = 65536 d1 + 256 d2 + d3), so that the down projection runs on the same integer matrix instruction and h is off by 2^-22 of its block's largest value.
+// The six-call path quantises h to int8 in between; here a block of 32 values of h is integers Q times a power of two, in three int8 digits
+// (Q = 65536 d1 + 256 d2 + d3, |Q| <= 8355711), so that the down projection runs on the same integer matrix instruction and h is off by 2^-23 of its block's
+// largest value, half a unit: about what a single f32 operation is off by.
 //
 // Bound by the bytes of the experts that the tokens reach, each read once.  Both kernels work on 16 weight rows x one superblock per warp (lane
 // g = lane / 4, t = lane % 4 holds bytes 8t .. 8t+7 of each block of rows g and g + 8).  A warp has a ring of such pieces of its own in shared memory,
@@ -357,8 +358,9 @@ __device__ __forceinline__ void up_epilogue(const MoeArgs& p, const Routed& s, c
   const uint32_t most = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(h) & 0x7FFFFFFFu);  // (a NaN is above all numbers here)
   const int ex = max((int)(most >> 23), 1) - 127;                                           // |h| < 2^(ex + 1)
   const bool none = most >= 0x7F800000u;
-  const int up1 = min(21 - ex, 100);
-  const int Q = none ? 0 : __float2int_rn(h * __int_as_float((up1 + 127) << 23) * __int_as_float((21 - ex - up1 + 127) << 23));
+  // a unit of 2^(ex - 22), or twice that where the largest value would need more than three digits hold: M / 2 (M its 24 bits, 2^23 .. 2^24) rounded is above 127 * 65793
+  const int bits = (most & 0x7FFFFFu) <= 0x7EFEFEu ? 22 : 21, up1 = min(bits - ex, 100);
+  const int Q = none ? 0 : __float2int_rn(h * __int_as_float((up1 + 127) << 23) * __int_as_float((bits - ex - up1 + 127) << 23));
   const int d3 = (int8_t)Q, q1 = (Q - d3) >> 8, d2 = (int8_t)q1, d1 = (q1 - d2) >> 8;
   const int sum = __reduce_add_sync(0xFFFFFFFFu, Q);
   int8_t* hq = p.hq + (size_t)pair * 3 * p.F + f0 + lane;
@@ -366,7 +368,7 @@ __device__ __forceinline__ void up_epilogue(const MoeArgs& p, const Routed& s, c
   hq[p.F] = (int8_t)d2;
   hq[2 * p.F] = (int8_t)d3;
   if (lane == 0) {
-    const float unit_of = none ? __int_as_float(0x7FC00000) : ldexpf(1.0f, ex - 21);
+    const float unit_of = none ? __int_as_float(0x7FC00000) : ldexpf(1.0f, ex - bits);
     p.hs[(size_t)pair * per + f0 / 32] = unit_of;
     p.hsum[(size_t)pair * per + f0 / 32] = unit_of * (float)sum;
   }

@@ -275,3 +275,36 @@ def test_refuses_a_first_expert_that_no_sum_holds(izb, torch):
         with pytest.raises(izb.IzbError) as e:
             izb.moe_layer(b.wg, b.wu, b.wd, b.aq, b.asc, b.logits, 2, x=b.x, e0=e0)
         assert e.value.status == -2
+
+
+def one_hot(N, K, at, d, q=1):
+    """Q8_0 rows with one value each: row n has d[n] * q[n] at at[n]."""
+    w = np.zeros((N, K // 32, 34), np.uint8)
+    n = np.arange(N)
+    w[n, at // 32, 0:2] = np.asarray(d, np.float16).reshape(-1, 1).view(np.uint8).reshape(N, 2)
+    w[n, at // 32, 2 + at % 32] = np.broadcast_to(np.asarray(q, np.int8), (N,)).view(np.uint8)
+    return w.reshape(N, -1)
+
+
+@pytest.mark.parametrize("size", [2.0 ** -90, 2.0 ** -20, 1.0, 2.0 ** 60])
+def test_how_exactly_h_is_held(izb, torch, size):
+    """Gate 64 (its silu is 64 to the last bit), up rows and down rows of one value each: the outputs are h as the second kernel gets it.  h is off by half a
+    unit, and a unit is 2^-22 of the power of two below the block's largest value M * 2^e -- or twice that, but then M > 0xFEFEFE, so that it is 2^-22 / 0.996 of
+    the largest value itself at most."""
+    F = E = 256
+    rng = np.random.default_rng(int(np.log2(size)) + 100)
+    most = np.array([0x800000, 0xFEFEFE, 0xFEFEFF, 0xFEFF00, 0xFFFFFF, 0x800001, 0x900000 + rng.integers(0x100000), 0xC00000 + rng.integers(0x100000)], np.float64)
+    asc = np.zeros((8, 16), np.float32)
+    asc[:, 0] = most * 2.0 ** -23 * size * 2.0 ** rng.integers(-3, 4, 8)
+    asc[0, 0] = 1.0  # (the gate's)
+    aq = np.zeros((16, E), np.int8)
+    aq[0, 0], aq[0, 1::32] = 64, 1
+    c = np.arange(F)
+    d = rng.uniform(-1, 1, F).astype(np.float16)
+    d[::32] = rng.choice([-1, 1], F // 32)  # each block's largest
+    h = 64.0 * (d.astype(np.float32) * asc[c // 32, 0]).astype(np.float64)
+    wg, wu, wd = (izb.Weight(8, w, 256, 256, n_mats=1) for w in (one_hot(F, E, 0 * c, np.ones(F)), one_hot(F, E, 32 * (c // 32) + 1, d), one_hot(E, F, c, np.ones(E))))
+    cu = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()
+    got = izb.moe_layer(wg, wu, wd, cu(aq), cu(asc), torch.zeros((1, 1), device="cuda"), 1).cpu().numpy()[0].astype(np.float64)
+    off = np.abs(got - h).reshape(-1, 32).max(1) / np.abs(h).reshape(-1, 32).max(1)
+    assert (off <= 2.0 ** -23 / 0.996).all(), off * 2.0 ** 23
