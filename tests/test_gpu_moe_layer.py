@@ -308,3 +308,32 @@ def test_how_exactly_h_is_held(izb, torch, size):
     got = izb.moe_layer(wg, wu, wd, cu(aq), cu(asc), torch.zeros((1, 1), device="cuda"), 1).cpu().numpy()[0].astype(np.float64)
     off = np.abs(got - h).reshape(-1, 32).max(1) / np.abs(h).reshape(-1, 32).max(1)
     assert (off <= 2.0 ** -23 / 0.996).all(), off * 2.0 ** 23
+
+
+@pytest.mark.parametrize("T,E,F,NE,NU,qt,qd,joined", [
+    (16, 512, 256, 40, 32, 12, 12, True),    # the most choices of a token
+    (5, 256, 512, 17, 17, 8, 8, False),      # every expert, more of them than half a warp
+    (12, 2048, 768, 64, 8, 12, 12, False),
+    (8, 768, 2560, 24, 20, 12, 8, True),
+])
+def test_on_average(izb, torch, T, E, F, NE, NU, qt, qd, joined):
+    """Off on average, as a share of the result: h is off by a unit / sqrt(12) per value, a unit being 2^-22 of its block's largest value at most, and 32 values whose largest is M have
+    a norm of M at least: sqrt(32 / 12) 2^-22 = 6.6 * 2^-24.  The roundings of the sums, 2^-24 of a partial sum each, add up as the square root of their number:
+    a warp's superblocks, three roundings each, and the joins, of gate and up, then of down, and the combine's."""
+    b = Block(izb, torch, T, E, F, NE, NU, qt, qd, joined, seed=NE)
+    want = b.want()
+    limit = 2.0 ** -24 * (6.6 + (2 * (3 * E / 256 / 4 + 12) + 3 * F / 256 + 12 + 2 * NU) ** 0.5)
+    got = b.call().cpu().numpy().astype(np.float64)
+    assert np.linalg.norm(got - want) / np.linalg.norm(want) <= limit
+
+
+def test_ties_and_choices_of_no_weight(izb, torch):
+    """Compared with the 64-bit result whatever it is: it is finite, the choices that are -inf have weight 0."""
+    b = Block(izb, torch, 12, 512, 256, 40, 4, 12, 8)
+    b.logits[0] = 0.0
+    b.logits[1] = -b.logits[0]
+    b.logits[2, 5:30] = 7.0
+    b.logits[3] = float("-inf")
+    b.logits[3, 17], b.logits[3, 3] = 0.0, -1.0
+    want = b.want()
+    assert np.isfinite(want).all() and rel(b.call(), want) <= TOL
