@@ -161,11 +161,27 @@ class Engine {
           "lora_add");
   }
   // the expert block of a decode step's rows (izb_moe_layer): x [cur_T][E] += the experts' weighted sum over the quantised activations; scratch
-  // holds moe_scratch(NU, F) bytes
+  // holds moe_scratch(NU, F) bytes.  A rank of the expert-parallel split names its first expert, and with `part` receives its share alone there
+  // (x is not looked at then)
   size_t moe_scratch(int NU, int F) const { return izb_moe_layer_scratch(cur_T_, NU, F); }
-  void moe_layer(const GpuWeight& gate, const GpuWeight* up, const GpuWeight& down, const float* logits, int ldl, int NE, int NU, const float* sh, float* x, void* scratch) {
+  void moe_layer(const GpuWeight& gate, const GpuWeight* up, const GpuWeight& down, const float* logits, int ldl, int NE, int NU, const float* sh, float* x, void* scratch,
+                 int e0 = 0, float* part = nullptr) {
     if (gate.K != cur_K_) throw std::runtime_error("moe_layer: the quantised activations do not match these experts");
-    check(izb_moe_layer(gate.h, up ? up->h : nullptr, down.h, aq_, asc_, cur_T_, cur_Mp_, logits, ldl, NE, NU, 0, sh, x, x, scratch, stream_), "moe_layer");
+    check(izb_moe_layer(gate.h, up ? up->h : nullptr, down.h, aq_, asc_, cur_T_, cur_Mp_, logits, ldl, NE, NU, e0, sh, part ? nullptr : x, part ? part : x, scratch, stream_),
+          "moe_layer");
+  }
+  // the requests' rules on the current rows' logits, in place (izb_logits_process, which has the arrays' meanings)
+  struct LogitRules {
+    const float* params = nullptr;
+    const int32_t *hist = nullptr, *hist_off = nullptr, *bias_ids = nullptr, *bias_off = nullptr, *mask_row = nullptr;
+    const float* bias = nullptr;
+    const uint32_t* mask = nullptr;
+    int n_hist = 0, n_bias = 0, mask_words = 0, n_masks = 0;
+  };
+  void logits_process(float* logits, int ld, int V, const LogitRules& r, int32_t* best, float* logz) {
+    check(izb_logits_process(logits, ld, logits, ld, cur_T_, V, r.params, r.hist, r.hist_off, r.n_hist, r.bias_ids, r.bias, r.bias_off, r.n_bias, r.mask, r.mask_words,
+                             r.n_masks, r.mask_row, best, logz, stream_),
+          "logits_process");
   }
 
   // tp_setup (zero/mgpu/engine_tp_shard.h:88): join the communicator; id128 from izb_tp_unique_id on rank 0
