@@ -8,7 +8,9 @@
 // would want 128 rows of one adapter per tile and its accumulators back through registers for the base; the tensor pipe is 46 % busy at most.)
 //
 // Measured (us; floor by bytes): one row of 5120 -> 5120, rank 16: 5.0 (0.06); 64 requests of one row, 32 adapters of ranks 8 to 64, 5120 -> 17408: 29 (8.0); 64 of
-// four rows, rank 32: 34 (9.2); 8192 rows, ranks 64 and 32, 5120 -> 17408: 245 (182), of which the second product 205 at 5.5 TB/s.
+// four rows, rank 32: 34 (9.2); 8192 rows, ranks 64 and 32, 5120 -> 17408: 265 (182; 245 in a graph of such calls alone), of which
+// the second product 205 at 5.5 TB/s.  Off by, against 64 bits, of the norm of the adapters' part, in 2^-24: single rows 2; up to 8 rows, rank 16 / 64 / 256, f16 2 / 3 / 6 and
+// bf16 2 / 4 / 10; prompts f16 3 / 4 / 12, bf16 2 / 5 / 15 -- a matrix instruction cuts its sums off, always towards zero, and the second product's are R / 16 per piece in a row.
 //
 // Two forms.  Decode rows (lora_few_kernel, up to 8 rows per segment on average): one launch and no memory for u.  A cluster of CTAs per tile of up to 8 rows
 // of a segment, each with a share of K; the partial sums meet in distributed shared memory, and each CTA goes on with its share of the outputs.
@@ -1055,6 +1057,8 @@ __global__ void __launch_bounds__(kThreads, 2) lora_outer_kernel(LoraArgs p, Row
 }
 
 constexpr int kMaxInner = 200 << 10;
+// The host knows how many rows and segments there are, not which segments are long or empty.  Where they are unlike the form that the average picks costs: 64 rows
+// of one request, 5120 -> 5120 at rank 64, 12 us alone and 20 beside 63 empty segments (as 64 single rows); 450 rows 19 alone and 54 with 63 single rows beside them.
 bool few_rows(int T, int n_seg) { return T <= 8 * (int64_t)n_seg; }
 
 }  // namespace

@@ -17,11 +17,12 @@
 // them writes it out for the second kernel, which reads it behind its wait for the first one: what kernels before this call wrote is visible to it from
 // there on only.
 //
-// Measured (us; the six calls / this; the floor by bytes), 128 experts of 768 over 2048, top 8, Q4_K: one token 26 / 18 (3.3), four 48 / 36, eight 88 / 55 (21),
-// 16 154 / 88, 32 208 / 143 (45); 60 experts of 1280 over 4096, top 4, five tokens 99 / 56.  Many tokens per expert are where the block-per-column form has nothing
-// to gain (it costs every token eight instructions): 8 experts, top 2, 32 tokens 47 / 55.  One token is latency: routing 2.6 us, first bytes of weights 2.4, the
+// Measured (us; the six calls / this; the floor by bytes), 128 experts of 768 over 2048, top 8, Q4_K: one token 26 / 16 (3.3), four 48 / 36, eight 88 / 57 (21),
+// 16 156 / 91, 32 211 / 150 (45); 60 experts of 1280 over 4096, top 4, five tokens 100 / 58.  Many tokens per expert are where the block-per-column form has nothing
+// to gain (it costs every token eight instructions): 8 experts, top 2, 32 tokens 47 / 57.  One token is latency: routing 2.6 us, first bytes of weights 2.4 in each kernel,
 // barriers.  Eight tokens: the first kernel's loop runs at 4.1 TB/s, the second one's at 2.9, both near 48 % of the issue slots with 16 warps per multiprocessor:
-// a superblock of gate and up takes about 560 instructions, of which decoding 6-bit scales is a fifth.
+// a superblock of gate and up takes about 560 instructions, of which decoding 6-bit scales is a fifth; the rest of the time is fixed latencies that 16 warps do
+// not cover.  The first kernel's 128 registers leave 12 (Q4_K) and 20 bytes (Q8_0) of a thread in local memory.
 // (Taken back: 24 warps per multiprocessor with gate and up one after the other and 80 registers, 55 -> 82 us; calling the routing and the epilogues once on
 // zeros so that their code is in the cache, 18 -> 23.)
 #include "izb_common.cuh"

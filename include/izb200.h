@@ -249,9 +249,11 @@ int izb_gemm(const izb_weight* w, int mat, const int8_t* d_aq, const float* d_as
  * d_ranks [n_adapters] (NULL: all R): adapters of lower rank; their rows of A and columns of B from the rank on are zeros.  Ranks outside 0..R are cut
  * to it.  d_seg [n_seg + 1]: row offsets, increasing (equal ones: an empty segment); what lies outside 0..T is cut off.  Rows before d_seg[0]
  * and behind the last segment are left as they were.  base: d_base [T][ldb] (its first column), d_base = d_C + c_off with ldb = ldc to add in place, or
- * NULL for zeros; rows of segments without an adapter receive the base.  Sums in f32 in an order that depends on the row's place in its segment's
- * tiles and the call's number of rows and segments alone, not on other rows' values.  A row whose inner sums are not all finite has no finite
- * outputs.  A, B, aq, asc 16-byte aligned, base and C any f32 address (16-byte aligned rows are faster).  d_scratch: izb_lora_scratch(dtype, R, T, n_seg) bytes (0 for
+ * NULL for zeros; rows of segments without an adapter receive the base.  Sums in f32 in an order that depends on the segment's length and rank, the row's
+ * place in it and the call's number of rows and segments alone, not on other rows' values.  A row whose inner sums are not all finite has no finite
+ * outputs.  How the rows are worked on follows from T and n_seg alone, on the understanding that segments are alike: single rows where T <= n_seg, tiles of 8 rows
+ * where T <= 8 n_seg, else of 64.  Empty segments count, so a table padded to a fixed number of segments, or one long prompt among single rows, gets right results
+ * but may read an adapter once per row or per 8 rows of the prompt: calls of their own for the prompts are faster there.  A, B, aq, asc 16-byte aligned, base and C any f32 address (16-byte aligned rows are faster).  d_scratch: izb_lora_scratch(dtype, R, T, n_seg) bytes (0 for
  * up to 8 rows per segment on average: then NULL will do), 16-byte aligned, the call's own until it has finished. */
 size_t izb_lora_scratch(int dtype, int R, int T, int n_seg);
 int izb_lora_add(int dtype, const void* d_A, const void* d_B, int n_adapters, int R, const int32_t* d_ranks, const float* d_scales, int N, int K,
@@ -351,7 +353,7 @@ int izb_moe_combine_ex(float* d_x, const float* d_y, const int32_t* d_inv, int T
  * rank's partial output); d_sh [T][K] and its gate (logit NE) NULL: no shared expert.  d_x, d_sh and d_out are contiguous [T][K]; d_out may be d_x
  * or d_sh.  d_scratch: izb_moe_layer_scratch(T, NU, F) bytes, 16-byte aligned, the call's own until it has finished.
  * h is not quantised to int8 on the way, as the six calls above do (izb_quantize_act between _gateup and _down): results agree with theirs to that rounding,
- * and are nearer to the exact ones.  It is for tokens that few others share an expert with: where eight and more do (32 tokens, 8 experts, 2 choices), the
+ * and are nearer to the exact ones (h is off by 2^-23 of the largest of its 32 values at most).  It is for tokens that few others share an expert with: where eight and more do (32 tokens, 8 experts, 2 choices), the
  * six calls are as fast or faster.  A token whose gate * up product is no finite number is NaN. */
 size_t izb_moe_layer_scratch(int T, int NU, int F);
 int izb_moe_layer(const izb_weight* wg, const izb_weight* wu, const izb_weight* wd, const int8_t* d_aq, const float* d_asc, int T, int Mp,
